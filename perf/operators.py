@@ -167,14 +167,25 @@ def run(st):
     return {"product": _product, "topk": _topk, "clip": _clip}[st["op"]](st)
 
 
+def _handles(st):
+    """What a program makes once for its buffers and tables: the descriptions of 8-bit matrices, the list of gradients."""
+    if "handles" not in st:
+        from tfrec_amd.device import QuantRows
+        if st["op"] == "product":
+            st["handles"] = QuantRows(st["Aq"], st["sa"], st["K"]), QuantRows(st["Bq"], st["sb"], st["K"])
+        elif st["op"] == "topk":
+            st["handles"] = QuantRows(st["Pq"], st["sp"], st["d"]), QuantRows(st["Qq"], st["sq"], st["d"])
+        else:
+            st["handles"] = _device().grad_list(st["grads"], out=st["outs"])
+    return st["handles"]
+
+
 def _product(st):
     if own:
-        from tfrec_amd.device import QuantRows
-        dev = _device()
-        a = QuantRows(st["Aq"], st["sa"], st["K"])
+        dev, (a, b) = _device(), _handles(st)
         if st["x"] != "i8":
             dev.quantize_rows(st["X"], out=a)
-        return {"C": dev.matmul_i8(a, QuantRows(st["Bq"], st["sb"], st["K"]), bias=st["biasv"], out=st["C"])}
+        return {"C": dev.matmul_i8(a, b, bias=st["biasv"], out=st["C"])}
     K = st["K"]
     if st["x"] == "i8":
         a, sa = st["Aq"][:, :K].float(), st["sa"]
@@ -190,9 +201,8 @@ def _product(st):
 
 def _topk(st):
     if own:
-        from tfrec_amd.device import QuantRows
-        ids, scores = _device().score_topk_i8(QuantRows(st["Pq"], st["sp"], st["d"]), QuantRows(st["Qq"], st["sq"], st["d"]), st["b"], st["users"],
-                                              st["k"], train=st["train"], out_ids=st["ids"], out_scores=st["scores"])
+        p, q = _handles(st)
+        ids, scores = _device().score_topk_i8(p, q, st["b"], st["users"], st["k"], train=st["train"], out_ids=st["ids"], out_scores=st["scores"])
         return {"ids": ids, "scores": scores}
     d, k, I = st["d"], st["k"], st["I"]
     users = st["users"].long()
@@ -215,7 +225,7 @@ def _topk(st):
 
 def _clip(st):
     if own:
-        _device().clip_grads(st["grads"], st["max_norm"], out=st["outs"], norm=st["norm"])
+        _device().clip_grads(_handles(st), st["max_norm"], norm=st["norm"])
         return {"grads": st["out_flat"], "norm": st["norm"]}
     norm = torch.stack([x.double().square().sum() for x in st["grads"]]).sum().sqrt()
     scale = (st["max_norm"] / torch.clamp(norm, min=st["max_norm"])).float()
