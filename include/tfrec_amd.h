@@ -318,9 +318,58 @@ int tfrec_dns_select(tfrec_ctx *ctx, const float *d_P, const float *d_Q, const f
                      const int32_t *d_users, const int32_t *d_cand, int64_t n_pos, int C,
                      int32_t *d_out_neg);
 
+/* ---- bounded steps -------------------------------------------------------------------------- */
+#define TFREC_DT_F32 0
+#define TFREC_DT_BF16 1
+#define TFREC_DT_F16 2
+
+/* The gradients of the BPR loss without a step (the loss of tfrec_bpr_sgd_step, model/BPR.py:36-48): d_gP [U,d],
+ * d_gQ [I,d] and d_gb [I] are zeroed and receive the summed gradient of every row the batch touches (l2 terms
+ * included).  axpy(table, gradient, -lr) on the three tables is then bit for bit tfrec_bpr_sgd_step.  For steps
+ * that look at the whole gradient first (tfrec_grad_clip).  d_loss as there. */
+int tfrec_bpr_grads(tfrec_ctx *ctx, const float *d_P, const float *d_Q, const float *d_b, int64_t U, int64_t I, int d,
+                    const int32_t *d_users, const int32_t *d_pos, const int32_t *d_neg, int64_t B, float reg,
+                    float *d_gP, float *d_gQ, float *d_gb, double *d_loss);
+
+/* Global l2 norm over n tensors: *d_norm = sqrt(sum of all squares), squares and sums in float64.  h_grads[i] (device
+ * pointers in a host array; null where h_counts[i] is 0) holds h_counts[i] >= 0 values of type h_dtypes[i] (TFREC_DT_*),
+ * at any alignment of its type.  A tensor listed twice counts twice.  The host arrays are read before the call returns.
+ * No counterpart in the reference (tf.train optimizers step on what they get, model/BPR.py:48). */
+int tfrec_grad_norm(tfrec_ctx *ctx, int n, const void *const *h_grads, const int64_t *h_counts, const int *h_dtypes, float *d_norm);
+/* The same, and h_out[i] = h_grads[i] * s with s = max_norm / max(norm, max_norm), formed in float64 and rounded to
+ * float32; the product is rounded to float32, then to the tensor's type.  Within the bound s is 1 and every value is
+ * left as it is.  A norm that is infinite or not a number makes every value NaN.  h_out[i] may be
+ * h_grads[i]; apart from that no output may overlap another output or any gradient (TFREC_EINVAL).  d_norm (the norm
+ * before scaling) may be null.  max_norm: positive and finite.
+ * Both calls use fixed scratch of the context, never its workspace, and can be captured into a HIP graph; graphs
+ * captured from one context share that scratch and must not be replayed at the same time. */
+int tfrec_grad_clip(tfrec_ctx *ctx, int n, const void *const *h_grads, void *const *h_out, const int64_t *h_counts,
+                    const int *h_dtypes, float max_norm, float *d_norm);
+
+/* ---- 8-bit rows ------------------------------------------------------------------------------- */
+/* A matrix in 8-bit integers with one float32 scale per row: value = q * scale.  Rows are ldq bytes apart, ldq a
+ * multiple of 16 and at least d rounded up to 16, the base 16-byte aligned.  Scales are non-negative; a row with a
+ * NaN scale stands for a row that cannot be scored (its products are NaN).
+ * tfrec_quantize_rows_i8: scale = max|x| / 127 (float32, correctly rounded), q = the integer nearest to x / scale, ties
+ * to even, in [-127, 127]; columns d .. (d rounded up to 16) are set to 0.  A row of zeros has scale 0; a row that holds
+ * an infinity or NaN has scale NaN and zeros.  Source rows of type x_dtype (TFREC_DT_*), ldx elements apart: row
+ * d_rows[r] (ids below n_rows; an id outside is clamped and raises the bad-index flag), or row r where d_rows is null
+ * (n <= n_rows). */
+int tfrec_quantize_rows_i8(tfrec_ctx *ctx, const void *d_X, int x_dtype, int64_t n_rows, int64_t ldx, int64_t d,
+                           const int32_t *d_rows, int64_t n, int8_t *d_q, int64_t ldq, float *d_scale);
+/* C[m, n] = (sum_k A[m, k] B[n, k]) * sa[m] * sb[n] + bias[n] (d_bias may be null): the 8-bit form of the score matrix
+ * model/BPR.py:76-80 builds, or of any layer whose weights are kept in 8 bits.  The sum is exact in int32 (K <= 131071),
+ * then in float32: converted, times sa[m], times sb[n], plus bias[n], each rounded, and rounded once more where c_dtype
+ * (TFREC_DT_*) has 16 bits.  C rows are ldc >= N elements apart.  Columns of A and B from K on are not used.  Uses no
+ * workspace. */
+int tfrec_matmul_i8(tfrec_ctx *ctx, const int8_t *d_A, int64_t lda, const float *d_sa, int64_t M,
+                    const int8_t *d_B, int64_t ldb, const float *d_sb, int64_t N, int64_t K,
+                    const float *d_bias, void *d_C, int c_dtype, int64_t ldc);
+
 /* ---- evaluation ---------------------------------------------------------------------------- */
 #define TFREC_SCORE_F32 0    /* exact float32: score = fma chain over f ascending, starting at b[i] */
 #define TFREC_SCORE_BF16 1   /* operands rounded to bfloat16, float32 accumulation (MFMA)            */
+#define TFREC_SCORE_I8 2     /* rows of P and Q quantised by tfrec_quantize_rows_i8, then tfrec_score_topk_i8 */
 
 /* Scoring + top-k in factor form, never forming the dense [users, items] matrix that
  * model/BPR.py:76-80 (_predict) builds and evaluator/backend/cpp/evaluate.py:25-27 masks:
@@ -334,6 +383,19 @@ int tfrec_score_topk(tfrec_ctx *ctx, const float *d_P, const float *d_Q, const f
                      const int32_t *d_eval_users, int64_t n,
                      const int64_t *d_train_indptr, const int32_t *d_train_indices,
                      int k, int score_mode, int32_t *d_out_ids, float *d_out_scores);
+
+/* tfrec_score_topk on tables that are kept in 8 bits (tfrec_quantize_rows_i8): scores as tfrec_matmul_i8 forms them,
+ * score = ((float)sum * sp[user]) * sq[item] + b[item], each step rounded to float32; same order, masks and outputs.
+ * d_Pq: the user table [U, ldp], indexed by user id (an id outside is clamped and raises the bad-index flag), or, with
+ * p_compact = 1, the listed users' rows in list order (U >= n).  d_b [I] or null.  d <= 256, k <= 240, scales
+ * non-negative.  A user or item whose scale is NaN has no scores (no entry / never listed).
+ * Scratch comes from the context's workspace: call once, or tfrec_ctx_reserve, before capturing into a HIP graph. */
+int tfrec_score_topk_i8(tfrec_ctx *ctx, const int8_t *d_Pq, int64_t ldp, const float *d_sp, int64_t U, int p_compact,
+                        const int8_t *d_Qq, int64_t ldq, const float *d_sq, const float *d_b,
+                        int64_t I, int d, int64_t item_lo, int64_t item_hi,
+                        const int32_t *d_eval_users, int64_t n,
+                        const int64_t *d_train_indptr, const int32_t *d_train_indices,
+                        int k, int32_t *d_out_ids, float *d_out_scores);
 
 /* The same for a GPU that holds only its own item shard (rows item_id_lo .. item_id_lo +
  * n_shard_items of the full tables, stored from row 0) and receives the evaluated users' factor

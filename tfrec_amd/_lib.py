@@ -13,7 +13,8 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("TFREC_AMD_LIB") or os.path.join(_HERE, "lib", "libtfrec_amd.so")
 
 OK, EINVAL, EHIP, ENOMEM, EINDEX, EUNSUP = 0, -1, -2, -3, -4, -5
-SCORE_F32, SCORE_BF16 = 0, 1
+SCORE_F32, SCORE_BF16, SCORE_I8 = 0, 1, 2
+DT_F32, DT_BF16, DT_F16 = 0, 1, 2
 
 _p = C.c_void_p
 _i64 = C.c_int64
@@ -69,6 +70,12 @@ SIGNATURES = {
     "tfrec_items_dedup": (_int, [_p, _p, _p, _i64, _i64, _i64, _int, _p, _p, _p, _p, _p]),
     "tfrec_rows_gather": (_int, [_p, _p, _p, _i64, _int, _p, _i64, _p, _p]),
     "tfrec_bpr_dense_grad_step": (_int, [_p, _int, _p, _p, _p, _p, _i64, _i64, _int, _p, _p, _p, _i64, _f, _f, _p]),
+    "tfrec_bpr_grads": (_int, [_p, _p, _p, _p, _i64, _i64, _int, _p, _p, _p, _i64, _f, _p, _p, _p, _p]),
+    "tfrec_grad_norm": (_int, [_p, _int, _p, _p, _p, _p]),
+    "tfrec_grad_clip": (_int, [_p, _int, _p, _p, _p, _p, _f, _p]),
+    "tfrec_quantize_rows_i8": (_int, [_p, _p, _int, _i64, _i64, _i64, _p, _i64, _p, _i64, _p]),
+    "tfrec_matmul_i8": (_int, [_p, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _i64, _p, _p, _int, _i64]),
+    "tfrec_score_topk_i8": (_int, [_p, _p, _i64, _p, _i64, _int, _p, _i64, _p, _p, _i64, _int, _i64, _i64, _p, _i64, _p, _p, _int, _p, _p]),
     "tfrec_axpy": (_int, [_p, _p, _p, _f, _i64]),
     "tfrec_apr_adagrad_step": (_int, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _int, _p, _p, _p, _i64,
                                       _f, _f, _f, _f, _p]),

@@ -26,9 +26,20 @@ int tfrec_ws_require(tfrec_ctx *ctx, size_t bytes)
 {
     if (bytes <= ctx->ws_bytes) return TFREC_OK;
     TF_REQUIRE(!ctx->ws_fixed, TFREC_ENOMEM, "the fixed scratch block holds %zu bytes, %zu needed", ctx->ws_bytes, bytes);
-    // grow: wait for work that may still use the old block, then replace it
+    // under capture nothing may be waited for or allocated: refused before the capture is spoilt
+    hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+    TF_HIP(hipStreamIsCapturing(ctx->stream, &cap));
+    TF_REQUIRE(cap == hipStreamCaptureStatusNone, TFREC_ENOMEM,
+               "the workspace holds %zu bytes, %zu needed: it cannot grow while the stream is captured (call tfrec_ctx_reserve, or the entry once, before)",
+               ctx->ws_bytes, bytes);
+    // grow: wait for work that may still use the old block, then replace it (a block that a captured graph names is kept)
     TF_HIP(hipStreamSynchronize(ctx->stream));
-    if (ctx->ws) TF_HIP(hipFree(ctx->ws));
+    if (ctx->ws && ctx->ws_in_graph) {
+        TF_REQUIRE(ctx->n_retired < (int)(sizeof(ctx->retired) / sizeof(ctx->retired[0])), TFREC_ENOMEM,
+                   "the workspace grew too often beside captured graphs: reserve it for the largest call first");
+        ctx->retired[ctx->n_retired++] = ctx->ws;
+        ctx->ws_in_graph = false;
+    } else if (ctx->ws) TF_HIP(hipFree(ctx->ws));
     ctx->ws = nullptr;
     ctx->ws_bytes = 0;
     const size_t want = tf_align(bytes + bytes / 8, 1 << 20);
@@ -38,6 +49,15 @@ int tfrec_ws_require(tfrec_ctx *ctx, size_t bytes)
         return TFREC_ENOMEM;
     }
     ctx->ws_bytes = want;
+    return TFREC_OK;
+}
+
+int tfrec_note_capture(tfrec_ctx *ctx)
+{
+    if (ctx->ws_in_graph) return TFREC_OK;
+    hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+    TF_HIP(hipStreamIsCapturing(ctx->stream, &cap));
+    ctx->ws_in_graph = cap != hipStreamCaptureStatusNone;
     return TFREC_OK;
 }
 
@@ -77,6 +97,7 @@ extern "C" int tfrec_ctx_create(int device, void *hip_stream, tfrec_ctx **out)
     auto fail = [&](int code, const char *what, hipError_t e) {
         tfrec_set_error("%s: %s", what, hipGetErrorString(e));
         if (c->d_flags) (void)hipFree(c->d_flags);
+        if (c->d_small) (void)hipFree(c->d_small);
         if (c->own_stream) (void)hipStreamDestroy(c->stream);
         delete c;
         return code;
@@ -90,6 +111,8 @@ extern "C" int tfrec_ctx_create(int device, void *hip_stream, tfrec_ctx **out)
     }
     hipError_t e = hipMalloc((void **)&c->d_flags, 256);
     if (e != hipSuccess) { c->d_flags = nullptr; return fail(TFREC_ENOMEM, "hipMalloc(flags)", e); }
+    e = hipMalloc((void **)&c->d_small, TFREC_SMALL_BYTES);
+    if (e != hipSuccess) { c->d_small = nullptr; return fail(TFREC_ENOMEM, "hipMalloc(scratch)", e); }
     e = hipMemsetAsync(c->d_flags, 0, 256, c->stream);
     if (e != hipSuccess) return fail(TFREC_EHIP, "hipMemset(flags)", e);
     // (a failure to find the fixed scratch array only disables the no-allocation step, which then reports it)
@@ -104,6 +127,8 @@ extern "C" int tfrec_ctx_destroy(tfrec_ctx *ctx)
     (void)hipSetDevice(ctx->device);
     (void)hipStreamSynchronize(ctx->stream);
     if (ctx->ws) (void)hipFree(ctx->ws);
+    for (int i = 0; i < ctx->n_retired; ++i) (void)hipFree(ctx->retired[i]);
+    if (ctx->d_small) (void)hipFree(ctx->d_small);
     if (ctx->d_flags) (void)hipFree(ctx->d_flags);
     if (ctx->h_pinned) (void)hipHostFree(ctx->h_pinned);
     for (hipEvent_t e : ctx->marks)

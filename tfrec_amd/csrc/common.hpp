@@ -64,6 +64,10 @@ struct tfrec_ctx {
     char *ws = nullptr;          // device workspace
     size_t ws_bytes = 0;
     size_t ws_used = 0;          // bump pointer, reset at the start of every entry point
+    bool ws_in_graph = false;    // a call that was captured into a HIP graph uses the workspace: its blocks then stay until destroy
+    void *retired[16] = {};      // blocks the workspace grew out of while a graph may still name them
+    int n_retired = 0;
+    char *d_small = nullptr;     // TFREC_SMALL_BYTES of scratch that never moves (partial sums of the gradient norm)
     bool ws_fixed = false;       // the workspace is a borrowed block of fixed size: never grown, never freed
     uint32_t *d_flags = nullptr; // sticky device-side error flags (4 bytes, separate allocation)
     void *h_pinned = nullptr;    // small pinned staging buffer for host outputs
@@ -80,6 +84,8 @@ struct tfrec_ctx {
     int n_marks = 0;
 };
 
+static constexpr size_t TFREC_SMALL_BYTES = 32 << 10;
+
 // Records a named timing mark on the stream when profiling is on (no-op otherwise).
 void tfrec_mark(tfrec_ctx *ctx, const char *name);
 void tfrec_marks_reset(tfrec_ctx *ctx);
@@ -93,6 +99,8 @@ int tfrec_ctx_enter(tfrec_ctx *ctx);
 int tfrec_ws_require(tfrec_ctx *ctx, size_t bytes);
 // Carves `bytes` (256-byte aligned) out of the workspace; tfrec_ws_require must have covered it.
 void *tfrec_ws_take(tfrec_ctx *ctx, size_t bytes);
+// Called by entry points whose launches may be captured: from then on the workspace's blocks outlive their replacement.
+int tfrec_note_capture(tfrec_ctx *ctx);
 int tfrec_pinned_require(tfrec_ctx *ctx, size_t bytes);
 
 static inline size_t tf_align(size_t x, size_t a = 256) { return (x + a - 1) / a * a; }

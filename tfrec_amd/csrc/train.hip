@@ -59,6 +59,7 @@ struct BprParams {
     float *P2;
     uint8_t *ver;
     float *gQ, *gb;      // where the item pass leaves gradient sums when it does not apply them (may alias Q, b)
+    float *gP;           // where the user pass leaves gradient sums when it does not apply them (UGRAD)
     float *stage;        // [B, d] pre-step P[u] of every triple
     float *sbuf;         // [B]    s = sigma(-(x + 1e-7)) of every triple
     const uint2 *pair;   // [B]    (i, j) of every triple, range-checked
@@ -70,7 +71,8 @@ struct BprParams {
 };
 
 // VER: the user table is versioned (see BprParams): no pre-step rows are staged for the item pass.
-template <int LPR_, int NCH_, int VEC_, bool FULL_, bool LOSS, bool VER = false, bool SHORT = false>
+// UGRAD: the summed gradient of every distinct user goes to its row of gP, P stays as it is (plain table only).
+template <int LPR_, int NCH_, int VEC_, bool FULL_, bool LOSS, bool VER = false, bool SHORT = false, bool UGRAD = false>
 struct BprUserPol {
     enum { LPR = LPR_, NCH = NCH_, VEC = VEC_, DEPTH = TF_DEPTH_USER, SHORT_TILES = SHORT };
     using RowT = Row<LPR_, NCH_, VEC_>;
@@ -136,6 +138,10 @@ struct BprUserPol {
         float *dst = VER ? (v ? a.P : a.P2) : a.P;
         const RowT p = seg ? seg->p : RowT::load(src + off, gl, DM::nchunk(a.nchunk));
         const float nreg = (float)acc.cnt * a.reg, lr = a.lr;
+        if constexpr (UGRAD) {
+            p.map2(acc.v, [=](float pv, float av) { return fmaf(nreg, pv, -av); }).store(a.gP + off, gl, DM::nchunk(a.nchunk));
+            return;
+        }
         const RowT out = p.map2(acc.v, [=](float pv, float av) { return fmaf(-lr, fmaf(nreg, pv, -av), pv); });
         out.store(dst + off, gl, DM::nchunk(a.nchunk));
         // The row now lives in the other buffer.  apply() runs once per distinct user of the batch (in the tile kernel
@@ -862,17 +868,17 @@ struct ItemChunks {
 // plain layout (the pre-step user rows are then staged for the item pass)
 static int bpr_passes(tfrec_ctx *ctx, const tfrec_batch_slot &sl, float *d_P, float *d_Q, float *d_b, int64_t U, int d,
                       float lr, float reg, double *d_loss, bool item_grad_only = false, float *d_gQ = nullptr, float *d_gb = nullptr,
-                      const tfrec_utable *ut = nullptr, const ItemChunks *chunks = nullptr)
+                      const tfrec_utable *ut = nullptr, const ItemChunks *chunks = nullptr, float *d_gP = nullptr)
 {
     const int64_t B = sl.B;
     const int64_t k0 = sl.next_k;                 // which of the slot's batches this step consumes
     const uint32_t *keys = sl.keys + 3 * B * k0, *vals = sl.vals + 3 * B * k0;
     RowCfg cfg;
-    TF_REQUIRE(pick_cfg(d, all_aligned16({d_P, d_Q, ut ? ut->P2 : nullptr}), &cfg), TFREC_EUNSUP, "factor size d=%d is not supported (max 256)", d);
+    TF_REQUIRE(pick_cfg(d, all_aligned16({d_P, d_Q, ut ? ut->P2 : nullptr, d_gP, d_gP ? d_gQ : nullptr}), &cfg), TFREC_EUNSUP, "factor size d=%d is not supported (max 256)", d);
     StepWs w;
     const bool short_tiles = B <= SHORT_TILES_MAX_B;
     TF_TRY(step_ws_carve(ctx, B, d, cfg, &w, ut == nullptr, short_tiles));
-    BprParams a{d_P, d_Q, d_b, ut ? ut->P2 : nullptr, ut ? ut->ver : nullptr, d_gQ ? d_gQ : d_Q, d_gb ? d_gb : d_b, w.stage, w.sbuf,
+    BprParams a{d_P, d_Q, d_b, ut ? ut->P2 : nullptr, ut ? ut->ver : nullptr, d_gQ ? d_gQ : d_Q, d_gb ? d_gb : d_b, d_gP, w.stage, w.sbuf,
                 sl.pair + B * k0, sl.users_raw + B * k0, (uint32_t)U, d, d / cfg.vec, lr, reg, sl.kmask};
     const bool want_loss = d_loss != nullptr;
     int64_t *d_bounds = nullptr;
@@ -884,6 +890,19 @@ static int bpr_passes(tfrec_ctx *ctx, const tfrec_batch_slot &sl, float *d_P, fl
         TF_HIP(hipGetLastError());
     }
     auto passes = [&]<int LPR, int NCH, int VEC, bool FULL, bool VER, bool SHORT>() -> int {
+        if constexpr (!VER) {
+            if (d_gP) {
+                // gradients only: the loss terms ride along whether they are wanted or not (one instantiation)
+                TF_TRY(run_pass(ctx, BprUserPol<LPR, NCH, VEC, FULL, true, false, SHORT, true>{a}, w, keys, vals, 0, B, w.n_tiles_u, w.blocks_u, true,
+                                "user_tile", "user_fixup"));
+                if (want_loss) {
+                    loss_finalize_kernel<2><<<1, 256, 0, ctx->stream>>>(w.loss_part, w.blocks_u, d_loss);
+                    TF_HIP(hipGetLastError());
+                }
+                return run_pass(ctx, BprItemPol<LPR, NCH, VEC, FULL, true, false, SHORT>{a}, w, keys, vals, B, 2 * B, w.n_tiles_i, w.blocks_i, false,
+                                "item_tile", "item_fixup");
+            }
+        }
         if (want_loss) {
             TF_TRY(run_pass(ctx, BprUserPol<LPR, NCH, VEC, FULL, true, VER, SHORT>{a}, w, keys, vals, 0, B, w.n_tiles_u, w.blocks_u, true,
                             "user_tile", "user_fixup"));
@@ -1264,6 +1283,39 @@ static int dense_grad_step_impl(tfrec_ctx *ctx, int slot, float *d_P, const floa
         sl.B = -1;
     }
     return rc;
+}
+
+__global__ __launch_bounds__(256) void zero_tables_kernel(float *__restrict__ x, int64_t nx, float *__restrict__ y, int64_t ny, float *__restrict__ z, int64_t nz)
+{
+    const int64_t stride = (int64_t)gridDim.x * 256, t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    for (int64_t i = t; i < nx; i += stride) x[i] = 0.f;
+    for (int64_t i = t; i < ny; i += stride) y[i] = 0.f;
+    for (int64_t i = t; i < nz; i += stride) z[i] = 0.f;
+}
+
+// The gradients of the step without the step: user and item sums of the touched rows in zeroed tables.
+extern "C" int tfrec_bpr_grads(tfrec_ctx *ctx, const float *d_P, const float *d_Q, const float *d_b, int64_t U, int64_t I, int d,
+                               const int32_t *d_users, const int32_t *d_pos, const int32_t *d_neg, int64_t B, float reg, float *d_gP,
+                               float *d_gQ, float *d_gb, double *d_loss)
+{
+    TF_REQUIRE(d_gP && d_gQ && d_gb, TFREC_EINVAL, "null gradient table");
+    TF_REQUIRE(d_gP != d_P && d_gQ != d_Q && d_gb != d_b, TFREC_EINVAL, "gradients cannot replace the parameters");
+    TF_TRY(tfrec_ctx_enter(ctx));
+    TF_TRY(check_step_args(d_P, d_Q, d_b, U, I, d, d_users, d_pos, d_neg, B));
+    zero_tables_kernel<<<2048, 256, 0, ctx->stream>>>(d_gP, U * d, d_gQ, I * d, d_gb, I);
+    TF_HIP(hipGetLastError());
+    if (B == 0) {
+        if (d_loss) zero_tables_kernel<<<1, 256, 0, ctx->stream>>>((float *)d_loss, 4, nullptr, 0, nullptr, 0);
+        TF_HIP(hipGetLastError());
+        return TFREC_OK;
+    }
+    tfrec_marks_reset(ctx);
+    tfrec_mark(ctx, "start");
+    tfrec_batch_slot &sl = ctx->slots[2];
+    TF_TRY(slot_prepare(ctx, sl, ctx->stream, d_users, d_pos, d_neg, B, U, I));
+    tfrec_mark(ctx, "index");
+    return bpr_passes(ctx, sl, const_cast<float *>(d_P), const_cast<float *>(d_Q), const_cast<float *>(d_b), U, d, 0.f, reg, d_loss, true, d_gQ, d_gb,
+                      nullptr, nullptr, d_gP);
 }
 
 extern "C" int tfrec_bpr_dense_grad_step(tfrec_ctx *ctx, int slot, float *d_P, const float *d_Q, const float *d_b, float *d_G,

@@ -13,6 +13,7 @@ from . import _lib
 
 SCORE_F32 = _lib.SCORE_F32
 SCORE_BF16 = _lib.SCORE_BF16
+SCORE_I8 = _lib.SCORE_I8
 
 
 class DevArray:
@@ -111,6 +112,121 @@ class UserTable:
             self.close()
         except Exception:
             pass
+
+
+class QuantRows:
+    """A matrix in 8-bit integers with one float32 scale per row (value = ``q * scale``): ``q`` int8 [n, ld], ``scale``
+    float32 [n], both on the GPU and row-major; ``d`` columns are the matrix's, the others (up to ``ld``, a multiple of 16)
+    are padding.  ``Device.quantize_rows`` makes one; scales are non-negative."""
+
+    def __init__(self, q, scale, d):
+        shape = _shape(q)
+        if len(shape) != 2 or _dtype_name(q) != "int8":
+            raise ValueError("q must be an int8 matrix")
+        if _shape(scale) != (shape[0],) or _dtype_name(scale) != "float32":
+            raise ValueError("scale must be float32 [%d]" % shape[0])
+        d = int(d)
+        if d < 1 or shape[1] % 16 or shape[1] < (d + 15) // 16 * 16:
+            raise ValueError("%d columns need rows of a multiple of 16 bytes and at least %d, got %d" % (d, (d + 15) // 16 * 16, shape[1]))
+        self.q, self.scale, self.d = q, scale, d
+        self.shape = (shape[0], d)
+        self.ld = shape[1]
+        _ptr(q), _ptr(scale)            # device buffers, contiguous
+
+    def __len__(self):
+        return self.shape[0]
+
+
+class GradList:
+    """Gradient tensors (float32, bfloat16 or float16, contiguous, any shape) and, optionally, the tensors their scaled
+    values go to (same types and sizes; default: in place), checked once: a program makes one for its gradient buffers and
+    passes it to every ``grad_norm`` / ``clip_grads``.  It keeps the tensors alive."""
+
+    def __init__(self, dev, grads, out=None):
+        self.dev = dev
+        self.grads = list(grads)
+        self.out = self.grads if out is None else list(out)
+        n = len(self.grads)
+        if len(self.out) != n:
+            raise ValueError("%d outputs for %d gradients" % (len(self.out), n))
+        sizes, types, at, to = [], [], [], []
+        for g in self.grads:
+            sizes.append(_numel(g))
+            types.append(_dt(g))
+            at.append(_ptr_on(dev, g))
+        if out is None:
+            to = at
+        else:
+            for i, o in enumerate(self.out):
+                if _numel(o) != sizes[i] or _dt(o) != types[i]:
+                    raise ValueError("output %d has another type or size than its gradient" % i)
+                to.append(_ptr_on(dev, o))
+        self.n = n
+        self.c_grads = (C.c_void_p * max(n, 1))(*at)
+        self.c_out = (C.c_void_p * max(n, 1))(*to)
+        self.c_counts = (C.c_int64 * max(n, 1))(*sizes)
+        self.c_types = (C.c_int * max(n, 1))(*types)
+
+    def __len__(self):
+        return self.n
+
+
+_DT = {"float32": _lib.DT_F32, "bfloat16": _lib.DT_BF16, "float16": _lib.DT_F16}
+
+
+def _dtype_name(x):
+    return str(x.dtype).rsplit(".", 1)[-1]
+
+
+def _dt(x):
+    """Type code of a float32, bfloat16 or float16 buffer."""
+    try:
+        return _DT[_dtype_name(x)]
+    except KeyError:
+        raise ValueError("a float32, bfloat16 or float16 buffer is needed, got %s" % _dtype_name(x))
+
+
+def _numel(x):
+    n = 1
+    for s in x.shape:
+        n *= int(s)
+    return n
+
+
+def _ptr_on(dev, x):
+    """``_ptr`` of a buffer that has to live on ``dev``'s GPU."""
+    where = getattr(x, "device", None)
+    if where is not None and hasattr(x, "data_ptr"):
+        if where.type != "cuda" or where.index != dev.device:
+            raise ValueError("the tensor is on %s, the context on GPU %d" % (where, dev.device))
+    elif isinstance(x, (DevArray, DevView)) and x.dev.device != dev.device:
+        raise ValueError("the array is on GPU %d, the context on GPU %d" % (x.dev.device, dev.device))
+    return _ptr(x)
+
+
+def _rows2d(dev, x, name):
+    """(pointer, row pitch in elements) of a matrix whose rows are contiguous (a torch tensor may have a row pitch)."""
+    if len(_shape(x)) != 2:
+        raise ValueError("%s must be a matrix" % name)
+    if hasattr(x, "data_ptr") and not isinstance(x, (DevArray, DevView)):
+        if x.shape[1] > 1 and x.stride(1) != 1:
+            raise ValueError("%s: the values of a row must be contiguous" % name)
+        if x.device.type != "cuda" or x.device.index != dev.device:
+            raise ValueError("%s is on %s, the context on GPU %d" % (name, x.device, dev.device))
+        pitch = x.stride(0) if x.shape[0] > 1 else max(int(x.shape[1]), 1)
+        if pitch < x.shape[1]:
+            raise ValueError("%s: rows overlap" % name)
+        return x.data_ptr(), pitch
+    return _ptr_on(dev, x), _shape(x)[1]
+
+
+def _vector(dev, x, n, dtype, name):
+    """Pointer of a contiguous device vector of ``n`` values of ``dtype`` (None passes)."""
+    if x is None:
+        return None
+    if _shape(x) != (n,) or _dtype_name(x) != dtype:
+        raise ValueError("%s must be %s [%d]" % (name, dtype, n))
+    return _ptr_on(dev, x)
 
 
 def _ptr(x):
@@ -370,6 +486,73 @@ class Device:
         _lib.check(self.lib.tfrec_bpr_dense_grad_step(self.h, int(slot), _ptr(P), _ptr(Q), _ptr(b), _ptr(G), U, I, d, _ptr(users),
                                                       _ptr(pos), _ptr(neg), B, float(lr), float(reg), _ptr(loss)))
 
+    def bpr_grads(self, P, Q, b, users, pos, neg, reg, gP, gQ, gb, loss=None):
+        """The gradients of one minibatch's BPR loss (duplicates summed) in ``gP``, ``gQ``, ``gb``, which are overwritten
+        whole; the parameters stay.  ``axpy(table, gradient, -lr)`` on the three is ``bpr_sgd_step`` bit for bit."""
+        U, d = _shape(P)
+        I = _shape(Q)[0]
+        B = _shape(users)[0]
+        if _shape(gP) != (U, d) or _shape(gQ) != (I, d) or _shape(gb) != (I,):
+            raise ValueError("gradients need the shapes of their tables")
+        _lib.check(self.lib.tfrec_bpr_grads(self.h, _ptr(P), _ptr(Q), _ptr(b), U, I, d, _ptr(users), _ptr(pos), _ptr(neg), B, float(reg),
+                                            _ptr(gP), _ptr(gQ), _ptr(gb), _ptr(loss)))
+
+    # -- bounded steps ----------------------------------------------------------------------
+    def grad_list(self, grads, out=None):
+        """A ``GradList`` of the tensors: what a program that steps on the same buffers again and again keeps."""
+        return GradList(self, grads, out)
+
+    def grad_norm(self, grads, norm=None):
+        """Global l2 norm over the tensors (a sequence or a ``GradList``), float32 [1] on the GPU."""
+        g = grads if isinstance(grads, GradList) else GradList(self, grads)
+        norm = norm if norm is not None else self.empty(1, np.float32)
+        _lib.check(self.lib.tfrec_grad_norm(self.h, g.n, g.c_grads, g.c_counts, g.c_types, _vector(self, norm, 1, "float32", "norm")))
+        return norm
+
+    def clip_grads(self, grads, max_norm, out=None, norm=None):
+        """Scales every tensor by ``max_norm / max(norm, max_norm)``, norm = the global l2 norm over all of them: in place, or
+        into ``out`` (a sequence of tensors; with a ``GradList`` the list's own outputs).  Returns the norm before scaling,
+        float32 [1] on the GPU.  A norm that is not finite makes every value NaN."""
+        if isinstance(grads, GradList):
+            if out is not None:
+                raise ValueError("a GradList has its outputs already")
+            g = grads
+        else:
+            g = GradList(self, grads, out)
+        norm = norm if norm is not None else self.empty(1, np.float32)
+        _lib.check(self.lib.tfrec_grad_clip(self.h, g.n, g.c_grads, g.c_out, g.c_counts, g.c_types, float(max_norm),
+                                            _vector(self, norm, 1, "float32", "norm")))
+        return norm
+
+    # -- 8-bit rows -------------------------------------------------------------------------
+    def quantize_rows(self, X, rows=None, out=None):
+        """Rows of ``X`` (float32, bfloat16 or float16; all of them, or those listed in ``rows``, int32) in 8 bits with a scale
+        per row.  ``out``: a ``QuantRows`` of that many rows to fill; returns it."""
+        n_rows, d = _shape(X)
+        n = n_rows if rows is None else _shape(rows)[0]
+        xp, ldx = _rows2d(self, X, "X")
+        if out is None:
+            out = QuantRows(self.empty((n, (d + 15) // 16 * 16), np.int8), self.empty(n, np.float32), d)
+        if out.shape != (n, d):
+            raise ValueError("out holds %s, need %s" % (out.shape, (n, d)))
+        _lib.check(self.lib.tfrec_quantize_rows_i8(self.h, xp, _dt(X), n_rows, ldx, d, _vector(self, rows, n, "int32", "rows"), n,
+                                                   _ptr_on(self, out.q), out.ld, _ptr_on(self, out.scale)))
+        return out
+
+    def matmul_i8(self, A, B, bias=None, out=None):
+        """C[m, n] = sum_k A[m, k] B[n, k] of two ``QuantRows`` (scales applied) + bias[n], float32 unless ``out`` (a matrix whose
+        rows may have a pitch) is bfloat16 or float16.  The sums are exact in 32-bit integers."""
+        (M, K), (N, KB) = A.shape, B.shape
+        if K != KB:
+            raise ValueError("A has %d columns, B %d" % (K, KB))
+        out = out if out is not None else self.empty((M, N), np.float32)
+        if _shape(out) != (M, N):
+            raise ValueError("out must be [%d, %d]" % (M, N))
+        cp, ldc = _rows2d(self, out, "out")
+        _lib.check(self.lib.tfrec_matmul_i8(self.h, _ptr_on(self, A.q), A.ld, _ptr_on(self, A.scale), M, _ptr_on(self, B.q), B.ld,
+                                            _ptr_on(self, B.scale), N, K, _vector(self, bias, N, "float32", "bias"), cp, _dt(out), ldc))
+        return out
+
     def axpy(self, y, x, alpha, n=None):
         """y[i] = fma(alpha, x[i], y[i])."""
         n = int(n) if n is not None else int(np.prod(_shape(y)))
@@ -435,6 +618,25 @@ class Device:
         tp, ti = (train if train is not None else (None, None))
         _lib.check(self.lib.tfrec_score_topk(self.h, _ptr(P), _ptr(Q), _ptr(b), I, d, lo, hi, _ptr(eval_users), n, _ptr(tp), _ptr(ti),
                                              int(k), int(mode), _ptr(out_ids), _ptr(out_scores)))
+        return out_ids, out_scores
+
+    def score_topk_i8(self, P, Q, b, eval_users, k, train=None, item_range=None, compact=False, out_ids=None, out_scores=None):
+        """``score_topk`` on tables kept in 8 bits (``QuantRows``; see ``quantize_rows``): what ``matmul_i8`` with bias ``b`` (or None)
+        scores, ranked.  ``compact``: row r of ``P`` belongs to eval_users[r]; else ``P`` is the whole user table."""
+        (U, d), (I, dq) = P.shape, Q.shape
+        if d != dq:
+            raise ValueError("P has %d columns, Q %d" % (d, dq))
+        n, k = _shape(eval_users)[0], int(k)
+        lo, hi = item_range if item_range is not None else (0, I)
+        out_ids = out_ids if out_ids is not None else self.empty((n, k), np.int32)
+        out_scores = out_scores if out_scores is not None else self.empty((n, k), np.float32)
+        if _shape(out_ids) != (n, k) or _dtype_name(out_ids) != "int32" or _shape(out_scores) != (n, k) or _dtype_name(out_scores) != "float32":
+            raise ValueError("outputs must be int32 and float32 [%d, %d]" % (n, k))
+        tp, ti = (train if train is not None else (None, None))
+        _lib.check(self.lib.tfrec_score_topk_i8(self.h, _ptr_on(self, P.q), P.ld, _ptr_on(self, P.scale), U, 1 if compact else 0, _ptr_on(self, Q.q),
+                                                Q.ld, _ptr_on(self, Q.scale), _vector(self, b, I, "float32", "b"), I, d, int(lo), int(hi),
+                                                _vector(self, eval_users, n, "int32", "eval_users"), n, _ptr(tp), _ptr(ti), k,
+                                                _ptr_on(self, out_ids), _ptr_on(self, out_scores)))
         return out_ids, out_scores
 
     def score_topk_shard(self, P_rows, Q_shard, b_shard, item_id_lo, eval_users, k, train=None, mode=SCORE_F32,
