@@ -384,6 +384,19 @@ def test_topk_of_an_item_table_beyond_32_bit_offsets(dev):
         assert list(ids.numpy()[0]) == sorted(best.tolist())
 
 
+def test_topk_of_more_users_than_one_pass_holds(dev):
+    """30000 listed users (20 distinct ones) over 300k items: the table of best scores is cut into passes."""
+    case = topk_case(6, 20, 300000, 16, 30)
+    users = np.tile(np.arange(20, dtype=np.int32), 1500)
+    Pq, sp, Qq, sq, b, masks = case
+    for compact in (False, True):
+        P = quant_rows(Pq[users], sp[users], 16) if compact else quant_rows(Pq, sp, 16)
+        ids, sc = dev.score_topk_i8(P, quant_rows(Qq, sq, 16), torch.from_numpy(b).cuda(), torch.from_numpy(users).cuda(), 10, train=csr(masks),
+                                    compact=compact)
+        want = expected_topk(scores_f32(Pq, sp, Qq, sq, b), 10, masks)
+        assert (ids.numpy().reshape(1500, 20, 10) == want[0][None]).all() and (sc.numpy().reshape(1500, 20, 10) == want[1][None]).all()
+
+
 # --------------------------------------------------------------------------------------------------------- run together
 def test_product_then_dense_topk_equals_the_fused_form(dev):
     """The matrix of matmul_i8 ranked by topk_dense is what score_topk_i8 returns, bit for bit."""

@@ -1452,15 +1452,15 @@ extern "C" int tfrec_rank_metrics(tfrec_ctx *ctx, const int32_t *d_ids, const in
 }
 
 // evaluation scratch that depends only on the number of users and k (candidate lists, id and
-// score buffers, metric rows); the prepared item table comes on top for bf16 / padded scoring
+// score buffers, metric rows); the prepared item table comes on top for bf16 / padded scoring, the 8-bit rows and their
+// blocks' best scores for 8-bit scoring
 size_t tfrec_eval_scratch_bytes(int64_t n, int k)
 {
     int CAP = cap_for_k(k);
     if (!CAP) return 0;
     if (cap_for(k, true, 128) > CAP) CAP = cap_for(k, true, 128);      // whatever score mode and factor size the call will have
     const int64_t nc = n < (1 << 20) ? n : (1 << 20);
-    const size_t lists = tf_align(sizeof(uint64_t) * (size_t)nc * CAP), i8 = tfrec_score_i8_bytes_most(n, k);
-    return 2 * tf_align(4 * (size_t)n * k) + (i8 > lists ? i8 : lists) + metrics_host_need(n, k, 0, false) + 8192;
+    return 2 * tf_align(4 * (size_t)n * k) + tf_align(sizeof(uint64_t) * (size_t)nc * CAP) + metrics_host_need(n, k, 0, false) + 8192;
 }
 
 // workspace bytes one full evaluation needs

@@ -13,14 +13,13 @@ struct ScoreI8Args {
     const float *sq, *b;       // scales and biases by row of Qq; b may be null
     int d;
     int64_t item_lo, n_items;
-    int64_t split_items;       // items per grid.y slice
     int64_t id_offset;         // added to the row of Qq to form the reported id
     const int32_t *users;      // [n]
     int64_t n;
     const int64_t *train_indptr;
     const int32_t *train_indices;
     int k;
-    int32_t *out_ids;          // [splits, n, k]
+    int32_t *out_ids;          // [n, k]
     float *out_scores;
     uint32_t *flags;
 };
@@ -33,4 +32,3 @@ int tfrec_quantize_rows(tfrec_ctx *ctx, const void *d_X, int x_dtype, int64_t n_
 // Scores and ranks; scratch from the workspace above what is in use (score_i8.hip).
 int tfrec_score_i8(tfrec_ctx *ctx, ScoreI8Args a);
 size_t tfrec_score_i8_bytes(int64_t n, int64_t n_items, int k);        // its scratch
-size_t tfrec_score_i8_bytes_most(int64_t n, int k);                    // for any number of items
