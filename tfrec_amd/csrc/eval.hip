@@ -1156,7 +1156,7 @@ static int plan_score(const float *d_Q, int d, int64_t item_lo, int64_t item_hi,
 static size_t quantized_bytes(int64_t rows, int d) { return tf_align((size_t)rows * tf_align(d, 16)) + tf_align((size_t)rows * 4); }
 static size_t score_i8_need(int64_t n, int64_t n_items, int d, int k)
 {
-    return quantized_bytes(n, d) + quantized_bytes(n_items, d) + tfrec_score_i8_bytes(n, n_items, k) + 1024;
+    return quantized_bytes(n, d) + quantized_bytes(n_items, d) + tfrec_score_i8_bytes(n, n_items, d, k) + 1024;
 }
 
 static int score_topk_quantized(tfrec_ctx *ctx, const float *d_P, const float *d_Q, const float *d_b, int d, int64_t item_lo, int64_t item_hi,

@@ -7,11 +7,12 @@
 //
 // Up to SMALL_ITEMS items, one workgroup scores them all for its user and keeps the scores in registers
 // (score_small_i8_kernel).  Beyond that:
-//   1. score_max_i8_kernel: all scores on the matrix cores; of every 32 items (a block) only the best score of every user
-//      is kept: the table is read once however few the users are, and 1/32 of the scores is written.
-//   2. pick_i8_kernel, a workgroup per user: the k-th largest of the best scores of disjoint groups of blocks that hold no
-//      train item is a lower bound T of the user's k-th best score (k different rankable items reach it).  Only blocks whose
-//      best score reaches T can hold a listed item: k blocks and few more, which are scored again, item by item.
+//   1. score_max_i8_kernel: all scores on the matrix cores; of every 16 items (a cell: the items whose scores one lane holds)
+//      only an upper bound of the best score is kept for every user, and per user how far below its bound a cell's best
+//      score can be: the table is read once however few the users are, and 1/16 of the scores is written.
+//   2. pick_i8_kernel, a workgroup per user: the k-th largest of the bounds of disjoint groups of cells that hold no train
+//      item, less that distance, is a lower bound T of the user's k-th best score (k different rankable items reach it).
+//      Only cells whose bound reaches T can hold a listed item: k and few more, which are scored again, item by item.
 // Neither depends on the order of the items, and nothing is kept between calls.
 #include "i8_device.hpp"
 #include "score_i8.hpp"
@@ -21,7 +22,7 @@ typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
 typedef int32_t i32x16 __attribute__((ext_vector_type(16)));
 struct __attribute__((packed, aligned(4))) Float4 { float v[4]; };       // 16 bytes at the alignment of a float
 
-static constexpr int BLOCK = 32;               // items per block
+static constexpr int BLOCK = 32, CELL = 16;    // items per block (a matrix instruction's rows) and per cell
 static constexpr int SMALL_ITEMS = 4096;       // (16 scores per thread of score_small_i8_kernel)
 static constexpr uint32_t KEY_NONE = 0x007fffffu;      // orderable form of -inf: nothing below or at it is listed
 
@@ -37,40 +38,82 @@ __device__ __forceinline__ int64_t user_row(const ScoreI8Args &a, int64_t r, int
     return c;
 }
 
-// score of item `it` (row item_lo + it of the table) for the user row p; the row's bytes from column d on are left out
-__device__ __forceinline__ float score_item(const ScoreI8Args &a, const int8_t *__restrict__ p, float sp, int64_t it)
-{
-    const uint4 *__restrict__ q = reinterpret_cast<const uint4 *>(a.Qq + (a.item_lo + it) * a.ldq);
-    const int chunks = (a.d + 15) / 16;
-    int acc = 0;
-    for (int c = 0; c < chunks; ++c) {
-        const uint4 qv = q[c], pv = keep_below(reinterpret_cast<const uint4 *>(p)[c], 16 * c, a.d);
-        acc = __builtin_amdgcn_sdot4((int)qv.x, (int)pv.x, acc, false);
-        acc = __builtin_amdgcn_sdot4((int)qv.y, (int)pv.y, acc, false);
-        acc = __builtin_amdgcn_sdot4((int)qv.z, (int)pv.z, acc, false);
-        acc = __builtin_amdgcn_sdot4((int)qv.w, (int)pv.w, acc, false);
+// Scores of items by groups of LPI lanes (a power of two, at least the row's 16-byte chunks): a lane holds chunk lane % LPI of
+// the user's row and reads that chunk of an item's row, so that a wave's load covers whole rows.
+template <int LPI>
+struct RowDot {
+    uint4 p;
+    float sp;
+    int off;                   // byte offset of this lane's chunk in an item row
+    __device__ __forceinline__ void init(const ScoreI8Args &a, int64_t prow)
+    {
+        const int c = 16 * (threadIdx.x % LPI);
+        p = make_uint4(0, 0, 0, 0);
+        if (c < a.d) p = keep_below(*reinterpret_cast<const uint4 *>(a.Pq + prow * a.ldp + c), c, a.d);
+        off = c < a.d ? c : 0;                 // (a lane without a chunk reads the first, against zeros)
+        sp = a.sp[prow];
     }
-    return add_rounded(scaled_sum(acc, sp, a.sq[a.item_lo + it]), a.b ? a.b[a.item_lo + it] : 0.f);
-}
+    __device__ __forceinline__ uint4 load(const ScoreI8Args &a, int64_t it) const
+    {
+        return *reinterpret_cast<const uint4 *>(a.Qq + (a.item_lo + it) * a.ldq + off);
+    }
+    // the sum over the group's lanes, on all of them
+    __device__ __forceinline__ int dot(uint4 q) const
+    {
+        int s = __builtin_amdgcn_sdot4((int)q.x, (int)p.x, 0, false);
+        s = __builtin_amdgcn_sdot4((int)q.y, (int)p.y, s, false);
+        s = __builtin_amdgcn_sdot4((int)q.z, (int)p.z, s, false);
+        s = __builtin_amdgcn_sdot4((int)q.w, (int)p.w, s, false);
+        if constexpr (LPI > 1) s += __builtin_amdgcn_mov_dpp(s, 0xB1, 0xf, 0xf, true);       // quad_perm [1,0,3,2]
+        if constexpr (LPI > 2) s += __builtin_amdgcn_mov_dpp(s, 0x4E, 0xf, 0xf, true);       // quad_perm [2,3,0,1]
+        if constexpr (LPI > 4) s += __builtin_amdgcn_mov_dpp(s, 0x141, 0xf, 0xf, true);      // mirror of half a row of 16 lanes
+        if constexpr (LPI > 8) s += __builtin_amdgcn_mov_dpp(s, 0x140, 0xf, 0xf, true);      // mirror of the row
+        return s;
+    }
+    __device__ __forceinline__ float score(const ScoreI8Args &a, int acc, int64_t it) const
+    {
+        return add_rounded(scaled_sum(acc, sp, a.sq[a.item_lo + it]), a.b ? a.b[a.item_lo + it] : 0.f);
+    }
+    // Of 256 positions scored together, thread t owns this one: after LPI steps of 256 / LPI positions every thread has one.
+    static __device__ __forceinline__ int owned() { return (threadIdx.x % LPI) * (256 / LPI) + (threadIdx.x & 255) / LPI; }
+};
 
 // ------------------------------------------------------------------------------------------
-// step 1: the best score of every block of 32 items, for every user
+// step 1: a bound of the best score of every cell of 16 items, for every user
 // ------------------------------------------------------------------------------------------
 struct MaxArgs {
     ScoreI8Args s;
-    float *best;               // [n, pitch]; blocks beyond the last hold -inf
-    int64_t pitch;             // blocks per user row, a multiple of 8
+    float *bound;              // [n, pitch]
+    float *slack;              // [n, splits]: 1.6 sp sq, the largest over a split
+    int64_t pitch;             // cells per user row: 16 per group of 8 blocks
     int64_t groups;            // groups of 8 blocks
     int64_t groups_per_split;
     int user_groups, splits;
 };
 
+static constexpr float LOWEST = -3.402823466e38f;
+// A cell bound at or below this may stand for a cell without a score.
+static constexpr float NO_SCORE = LOWEST * (1.f - 0x1p-19f);
+
 // KS = steps of 32 columns, UW = sets of 32 users a wave holds (as the matrix instruction's B operand, resident; the items
-// are its A operand and come straight from memory, a block ahead).  A lane gets 16 scores of one user per block.
+// are its A operand and come straight from memory, a block ahead).  A lane gets 16 scores of one user per block: its cell
+// is items 8 g + 4 h + 0..3, g = 0..3, of the block.
+//
+// The vector work per score is what bounds this kernel once there are users enough, so the scores are formed in two
+// instructions instead of the definition's four: the accumulator starts at 1.5 * 2^23 as the BITS of a float, so that its
+// bits ARE the float 1.5 * 2^23 + sum (|sum| <= 256 * 2^14 = 2^22), and
+//     v = fma(fma(acc, sp, -1.5 * 2^23 * sp), sq, b).
+// Against the defined score e: the inner step is off by at most half an ulp of 1.5 * 2^23 sp (0.75 sp) and of the result
+// (2^-24 * 2^22 sp), the defined products by 2 * 2^-24 of theirs (0.5 sp sq at most), and both sums by half an ulp of what
+// they give: |v - e| <= 1.6 sp sq + 2^-22 |v|, plus a few steps of 2^-149.  A cell's bound is its largest v plus that
+// (with 2^-21 for its own rounding), its best e at least the bound less twice that; the first term, which does not show in
+// the bound, is kept per user and slice of the items.
+// Scales above 2^50 could leave float32's range in one form and not in the other: users and blocks that have such scales
+// take the definition itself.
 template <int KS, int UW>
-__global__ __launch_bounds__(256) void score_max_i8_kernel(MaxArgs m)
+__global__ __launch_bounds__(256, 2) void score_max_i8_kernel(MaxArgs m)
 {
-    __shared__ __align__(16) float out[4][UW][32][8];
+    __shared__ float out[4][UW][16][32];
     const ScoreI8Args &a = m.s;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 31, h = lane >> 5;
     // consecutive workgroups go to the 8 XCDs in turn: an XCD takes every 8th slice of the items, for all users one after
@@ -83,13 +126,18 @@ __global__ __launch_bounds__(256) void score_max_i8_kernel(MaxArgs m)
     const int64_t g0 = split * m.groups_per_split, g1 = g0 + m.groups_per_split < m.groups ? g0 + m.groups_per_split : m.groups;
 
     i32x4 pb[UW][KS];
-    float sp[UW];
+    float sp[UW], off_sp[UW], err_sp[UW], slack[UW];
+    bool wide_user = false;
 #pragma unroll
     for (int s = 0; s < UW; ++s) {
         const int64_t ur = (int64_t)ug * 32 * UW + 32 * s + r;
         int32_t id;
         const int64_t row = user_row(a, ur < a.n ? ur : a.n - 1, &id);
         sp[s] = a.sp[row];
+        off_sp[s] = -12582912.f * sp[s];
+        err_sp[s] = sp[s] == sp[s] ? 1.6f * sp[s] : 0.f;       // (a user without a scale has no scores to bound)
+        slack[s] = 0.f;
+        wide_user |= sp[s] > 0x1p50f;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
             const int c = 32 * ks + 16 * h;
@@ -132,6 +180,9 @@ __global__ __launch_bounds__(256) void score_max_i8_kernel(MaxArgs m)
                 }
         }
     };
+    i32x16 start;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) start[e] = 0x4B400000;
     Block cur;
     load(cur, g0 * 8);
     for (int64_t g = g0; g < g1; ++g) {
@@ -139,16 +190,36 @@ __global__ __launch_bounds__(256) void score_max_i8_kernel(MaxArgs m)
         for (int i = 0; i < 8; ++i) {
             Block next;
             load(next, g * 8 + i + 1);
+            float sqm = 0.f;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) sqm = fmaxf(sqm, cur.sq[e >> 2].v[e & 3]);
+            const bool wide = __ballot(wide_user || sqm > 0x1p50f) != 0;
+            i32x16 acc[2];
+            acc[0] = start;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) acc[0] = __builtin_amdgcn_mfma_i32_32x32x32_i8(cur.q[ks], pb[0][ks], acc[0], 0, 0, 0);
 #pragma unroll
             for (int s = 0; s < UW; ++s) {
-                i32x16 acc = {};
+                // the next set's products run beside this set's vector work
+                if (s + 1 < UW) {
+                    acc[(s + 1) & 1] = start;
 #pragma unroll
-                for (int ks = 0; ks < KS; ++ks) acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(cur.q[ks], pb[s][ks], acc, 0, 0, 0);
-                float mx = -INFINITY;
+                    for (int ks = 0; ks < KS; ++ks) acc[(s + 1) & 1] = __builtin_amdgcn_mfma_i32_32x32x32_i8(cur.q[ks], pb[s + 1][ks], acc[(s + 1) & 1], 0, 0, 0);
+                }
+                const i32x16 &x = acc[s & 1];
+                float mx = LOWEST, d = 0x1p-140f;
+                if (!wide) {
 #pragma unroll
-                for (int e = 0; e < 16; ++e) mx = fmaxf(mx, add_rounded(scaled_sum(acc[e], sp[s], cur.sq[e >> 2].v[e & 3]), cur.b[e >> 2].v[e & 3]));
-                mx = fmaxf(mx, __uint_as_float(swap32(__float_as_uint(mx), lane)));
-                if (h == 0) out[wave][s][r][i] = mx;
+                    for (int e = 0; e < 16; ++e) mx = fmaxf(mx, fmaf(fmaf(__int_as_float(x[e]), sp[s], off_sp[s]), cur.sq[e >> 2].v[e & 3], cur.b[e >> 2].v[e & 3]));
+                    d = fmaf(err_sp[s], sqm, d);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        mx = fmaxf(mx, add_rounded(scaled_sum(x[e] - 0x4B400000, sp[s], cur.sq[e >> 2].v[e & 3]), cur.b[e >> 2].v[e & 3]));
+                }
+                slack[s] = fmaxf(slack[s], d);
+                d = fmaf(fabsf(mx), 0x1p-21f, d);
+                out[wave][s][2 * i + h][r] = mx + d;
             }
             cur = next;
         }
@@ -157,15 +228,28 @@ __global__ __launch_bounds__(256) void score_max_i8_kernel(MaxArgs m)
 #pragma unroll
         for (int s = 0; s < UW; ++s) {
             const int64_t ur = (int64_t)ug * 32 * UW + 32 * s + r;
-            if (ur < a.n) *reinterpret_cast<float4 *>(m.best + ur * m.pitch + g * 8 + 4 * h) = *reinterpret_cast<const float4 *>(&out[wave][s][r][4 * h]);
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = out[wave][s][8 * h + j][r];
+            if (ur < a.n) {
+                float4 *to = reinterpret_cast<float4 *>(m.bound + ur * m.pitch + g * 16 + 8 * h);
+                to[0] = make_float4(v[0], v[1], v[2], v[3]);
+                to[1] = make_float4(v[4], v[5], v[6], v[7]);
+            }
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
     }
+#pragma unroll
+    for (int s = 0; s < UW; ++s) {
+        const int64_t ur = (int64_t)ug * 32 * UW + 32 * s + r;
+        slack[s] = fmaxf(slack[s], __uint_as_float(swap32(__float_as_uint(slack[s]), lane)));
+        if (h == 0 && ur < a.n) m.slack[ur * m.splits + split] = slack[s];
+    }
 }
 
 // ------------------------------------------------------------------------------------------
-// a workgroup's list of keys (256 threads)
+// a workgroup's list of keys (scored by 256 threads; NT threads in all)
 // ------------------------------------------------------------------------------------------
 static constexpr int LIST = 1024;
 struct GroupList {
@@ -173,22 +257,23 @@ struct GroupList {
     uint64_t kth;              // keys at or below it are not wanted
     int count;
     uint32_t hist[2][64];
-    uint32_t lo[4], hi[4];
-    int valid[4];
+    uint32_t lo[16], hi[16];
+    int valid[16];
 };
 
-// A lower bound of the k-th largest of the workgroup's orderable values (V per thread; values at or below KEY_NONE are
+// A lower bound of the k-th largest of the workgroup's orderable values (V per thread; values at or below `none` are
 // none): the lower edge of a bucket of a two-level histogram below the highest bit in which the values differ.
-// KEY_NONE + 1 if fewer than k values are held.
-template <int V>
-__device__ __forceinline__ uint32_t rank_bound(const uint32_t (&key)[V], int k, GroupList &g)
+// 0 if fewer than k values are held.
+template <int NT, int V>
+__device__ __forceinline__ uint32_t rank_bound(const uint32_t (&key)[V], uint32_t none, int k, GroupList &g)
 {
+    constexpr int NW = NT / 64;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     uint32_t lo = 0xffffffffu, hi = 0;
     int valid = 0;
 #pragma unroll
     for (int v = 0; v < V; ++v)
-        if (key[v] > KEY_NONE) {
+        if (key[v] > none) {
             lo = key[v] < lo ? key[v] : lo;
             hi = key[v] > hi ? key[v] : hi;
             valid += 1;
@@ -202,20 +287,21 @@ __device__ __forceinline__ uint32_t rank_bound(const uint32_t (&key)[V], int k, 
     if (lane == 0) { g.lo[wave] = lo; g.hi[wave] = hi; g.valid[wave] = valid; }
     if (threadIdx.x < 128) g.hist[threadIdx.x >> 6][threadIdx.x & 63] = 0;
     __syncthreads();
+    valid = 0;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < NW; ++w) {
         lo = g.lo[w] < lo ? g.lo[w] : lo;
         hi = g.hi[w] > hi ? g.hi[w] : hi;
+        valid += g.valid[w];
     }
-    valid = g.valid[0] + g.valid[1] + g.valid[2] + g.valid[3];
-    if (valid < k) return KEY_NONE + 1;
+    if (valid < k) return 0;
     if (lo == hi) return hi;
     const int top = 31 - __builtin_clz(lo ^ hi);
     const int s1 = top >= 5 ? top - 5 : 0;
     // level 1: six bits from the highest differing one down (all values share the bits above)
 #pragma unroll
     for (int v = 0; v < V; ++v)
-        if (key[v] > KEY_NONE) atomicAdd(&g.hist[0][(key[v] >> s1) & 63u], 1u);
+        if (key[v] > none) atomicAdd(&g.hist[0][(key[v] >> s1) & 63u], 1u);
     __syncthreads();
     auto level = [&](const uint32_t *hist, int want, int *above, int *in) {
         const int c = (int)hist[lane], incl = wave_prefix_sum(c), total = __builtin_amdgcn_readlane(incl, 63);
@@ -235,7 +321,7 @@ __device__ __forceinline__ uint32_t rank_bound(const uint32_t (&key)[V], int k, 
         const uint32_t mask = (1u << (s1 - s2)) - 1u;
 #pragma unroll
         for (int v = 0; v < V; ++v)
-            if (key[v] > KEY_NONE && key[v] >> s1 == cut >> s1) atomicAdd(&g.hist[1][(key[v] >> s2) & mask], 1u);
+            if (key[v] > none && key[v] >> s1 == cut >> s1) atomicAdd(&g.hist[1][(key[v] >> s2) & mask], 1u);
         __syncthreads();
         int above2, in2;
         cut |= level(g.hist[1], k - above, &above2, &in2) << s2;
@@ -291,84 +377,157 @@ __device__ __forceinline__ void group_finish(GroupList &g, const ScoreI8Args &a,
 }
 
 // ------------------------------------------------------------------------------------------
-// step 2: the blocks that can hold a listed item, scored again
+// step 2: the cells that can hold a listed item, scored again
 // ------------------------------------------------------------------------------------------
-static constexpr int SLICES = 1024;            // groups of blocks: block x belongs to slice x % SLICES
-static constexpr int CAND = 2048;              // blocks per round
+static constexpr int SLICES = 1024;            // groups of cells: cell y belongs to slice y % SLICES
+static constexpr int CAND = 2048;              // cells per round
 
-__global__ __launch_bounds__(256) void pick_i8_kernel(MaxArgs m)
+// first item of cell y, and item e of it
+__device__ __forceinline__ int64_t cell_first(int64_t y) { return (y >> 1) * BLOCK + 4 * (y & 1); }
+__device__ __forceinline__ int64_t cell_item(int64_t y, int e) { return cell_first(y) + 8 * (e >> 2) + (e & 3); }
+
+// NT = 256 threads, or 1024 where there are few users and one workgroup's time is the call's; LPI: see RowDot
+template <int NT, int LPI>
+__global__ __launch_bounds__(NT) void pick_i8_kernel(MaxArgs m)
 {
     __shared__ GroupList g;
     __shared__ uint32_t cand[CAND];
     __shared__ uint16_t slices[SLICES];
     __shared__ uint8_t train[SLICES];
     __shared__ int n_slices, n_cand;
+    __shared__ float slack;
+    constexpr int V = SLICES / NT;
     const ScoreI8Args &a = m.s;
     const int tid = threadIdx.x;
     const int64_t r = blockIdx.x;
     int32_t user;
     const int64_t prow = user_row(a, r, &user);
-    const int8_t *__restrict__ p = a.Pq + prow * a.ldp;
-    const float sp = a.sp[prow];
+    RowDot<LPI> dot;
+    dot.init(a, prow);
     const int64_t mlo = a.train_indptr ? a.train_indptr[user] : 0, mhi = a.train_indptr ? a.train_indptr[user + 1] : 0;
     const int64_t id0 = a.id_offset + a.item_lo;
-    const int64_t blocks = (a.n_items + BLOCK - 1) / BLOCK;
-    const float *__restrict__ best = m.best + r * m.pitch;
+    const uint32_t cells = 2u * (uint32_t)((a.n_items + BLOCK - 1) / BLOCK);
+    const float *__restrict__ bound = m.bound + r * m.pitch;
+    int64_t t = mlo + tid;
+    const int32_t train0 = t < mhi ? a.train_indices[t] : -1;
 
-    for (int i = tid; i < SLICES; i += 256) train[i] = 0;
+    // the largest bound of every slice
+    float mx[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) mx[v] = LOWEST;
+    constexpr int DEPTH = 16 / V > 4 ? 8 : 4;          // loads in flight: DEPTH * V
+    uint32_t y0 = 0;
+    for (; y0 + DEPTH * SLICES <= cells; y0 += DEPTH * SLICES) {
+        float w[DEPTH][V];
+#pragma unroll
+        for (int q = 0; q < DEPTH; ++q)
+#pragma unroll
+            for (int v = 0; v < V; ++v) w[q][v] = bound[y0 + q * SLICES + NT * v + tid];
+#pragma unroll
+        for (int q = 0; q < DEPTH; ++q)
+#pragma unroll
+            for (int v = 0; v < V; ++v) mx[v] = fmaxf(mx[v], w[q][v]);
+    }
+    {
+        float w[DEPTH][V];
+#pragma unroll
+        for (int q = 0; q < DEPTH; ++q)
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const uint32_t y = y0 + q * SLICES + NT * v + tid;
+                w[q][v] = y < cells ? bound[y] : LOWEST;
+            }
+#pragma unroll
+        for (int q = 0; q < DEPTH; ++q)
+#pragma unroll
+            for (int v = 0; v < V; ++v) mx[v] = fmaxf(mx[v], w[q][v]);
+    }
+    for (int i = tid; i < SLICES; i += NT) train[i] = 0;
     if (tid == 0) { g.count = 0; n_slices = 0; n_cand = 0; }
-    __syncthreads();
-    for (int64_t t = mlo + tid; t < mhi; t += 256) {
-        const int64_t i = a.train_indices[t] - id0;
-        if (i >= 0 && i < a.n_items) train[(i / BLOCK) % SLICES] = 1;
+    if (tid < 64) {
+        float w = 0.f;
+        for (int i = tid; i < m.splits; i += 64) w = fmaxf(w, m.slack[r * m.splits + i]);
+        for (int o = 32; o > 0; o >>= 1) w = fmaxf(w, __shfl_xor(w, o, 64));
+        if (tid == 0) slack = w;
     }
     __syncthreads();
-    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-    for (int64_t x0 = 0; x0 < blocks; x0 += SLICES) {
+    // (an index of any other sign or size is another shard's item)
+    auto mark = [&](int32_t id) {
+        const int64_t i = id - id0;
+        if (id >= 0 && i >= 0 && i < a.n_items) train[(2 * (i / BLOCK) + (i >> 2 & 1)) % SLICES] = 1;
+    };
+    mark(train0);
+    for (t += NT; t < mhi; t += NT) mark(a.train_indices[t]);
+    __syncthreads();
+    uint32_t key[V];
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
-            const int64_t x = x0 + 256 * v + tid;
-            if (x < blocks) mx[v] = fmaxf(mx[v], best[x]);
-        }
+    for (int v = 0; v < V; ++v) key[v] = train[NT * v + tid] ? 0u : f32_orderable(mx[v]);
+    const uint32_t cut = rank_bound<NT, V>(key, f32_orderable(NO_SCORE), a.k, g);
+    // T: the cut less what a bound may be off (twice the slack, and this arithmetic's rounding); without a cut all cells pass
+    float T = -INFINITY;
+    if (cut) {
+        const float c = fminf(orderable_f32(cut), -LOWEST);
+        T = c - 2.1f * slack - fabsf(c) * 0x1p-19f;
+        T = T > LOWEST ? T : -INFINITY;           // (also where T is not a number)
     }
-    uint32_t key[4];
 #pragma unroll
-    for (int v = 0; v < 4; ++v) key[v] = train[256 * v + tid] ? 0u : f32_orderable(mx[v]);
-    const uint32_t cut = rank_bound(key, a.k, g);
-#pragma unroll
-    for (int v = 0; v < 4; ++v)
-        if (f32_orderable(mx[v]) >= cut) slices[atomicAdd(&n_slices, 1)] = (uint16_t)(256 * v + tid);
-    if (tid == 0) g.kth = ((uint64_t)cut << 32) - 1;
+    for (int v = 0; v < V; ++v)
+        if (mx[v] >= T) slices[atomicAdd(&n_slices, 1)] = (uint16_t)(NT * v + tid);
+    if (tid == 0) g.kth = T > -INFINITY ? ((uint64_t)f32_orderable(T) << 32) - 1 : ((uint64_t)KEY_NONE << 32 | 0xffffffffu);
     __syncthreads();
 
-    const uint32_t per = (uint32_t)((blocks + SLICES - 1) / SLICES), total = (uint32_t)n_slices * per;      // (at most blocks + SLICES: below 2^27)
+    const uint32_t per = (cells + SLICES - 1) / SLICES, total = dot.sp == dot.sp ? (uint32_t)n_slices * per : 0u;
+    constexpr int ROUNDS = LPI <= 2 ? 4 : (LPI <= 8 ? 2 : 1);          // rounds of 256 items whose rows are requested together
     for (uint32_t e0 = 0; e0 < total; e0 += CAND) {
         const uint64_t kth = g.kth;
-#pragma unroll
-        for (int i = 0; i < CAND / 256; ++i) {
-            const uint32_t e = e0 + 256 * i + tid;
+        for (uint32_t i = tid; i < CAND; i += NT) {
+            const uint32_t e = e0 + i;
             if (e < total) {
-                const int64_t x = slices[e / per] + (int64_t)(e % per) * SLICES;
-                // the block's best score under its lowest id: if that is not wanted, nothing in the block is
-                if (x < blocks && make_key(best[x], (int32_t)(id0 + x * BLOCK)) > kth) cand[atomicAdd(&n_cand, 1)] = (uint32_t)x;
+                const uint32_t y = slices[e / per] + (e % per) * SLICES;
+                // the cell's bound under its lowest id: if that is not wanted, nothing in the cell is
+                if (y < cells && make_key(bound[y], (int32_t)(id0 + cell_first(y))) > kth) cand[atomicAdd(&n_cand, 1)] = y;
             }
         }
         __syncthreads();
         const int c = n_cand;
-        for (int c0 = 0; c0 < c; c0 += 256 / BLOCK) {
-            const int at = c0 + tid / BLOCK;
-            bool pass = false;
-            uint64_t k64 = 0;
-            if (at < c) {
-                const int64_t it = (int64_t)cand[at] * BLOCK + tid % BLOCK;
-                if (it < a.n_items) {
-                    const float v = score_item(a, p, sp, it);
-                    k64 = make_key(v, (int32_t)(id0 + it));
-                    pass = v > -INFINITY && k64 > g.kth;
-                }
+        for (int c0 = 0; c0 < c * CELL; c0 += 256 * ROUNDS) {
+            int acc[ROUNDS];
+            if (tid < 256) {
+                uint4 q[ROUNDS][LPI];
+#pragma unroll
+                for (int o = 0; o < ROUNDS; ++o)
+#pragma unroll
+                    for (int j = 0; j < LPI; ++j) {
+                        const int i = c0 + 256 * o + j * (256 / LPI) + tid / LPI;
+                        int64_t it = i < c * CELL ? cell_item(cand[i / CELL], i % CELL) : 0;
+                        it = it < a.n_items ? it : 0;
+                        q[o][j] = dot.load(a, it);
+                    }
+#pragma unroll
+                for (int o = 0; o < ROUNDS; ++o)
+#pragma unroll
+                    for (int j = 0; j < LPI; ++j) {
+                        const int s = dot.dot(q[o][j]);
+                        if (tid % LPI == j) acc[o] = s;
+                    }
             }
-            group_append(g, pass, k64);
-            group_check(g, a.k, a.train_indices, mlo, mhi);
+#pragma unroll
+            for (int o = 0; o < ROUNDS; ++o) {
+                if (o > 0 && c0 + 256 * o >= c * CELL) break;
+                if (tid < 256) {
+                    const int i = c0 + 256 * o + RowDot<LPI>::owned();
+                    const int64_t it = i < c * CELL ? cell_item(cand[i / CELL], i % CELL) : a.n_items;
+                    bool pass = false;
+                    uint64_t k64 = 0;
+                    if (it < a.n_items) {
+                        const float v = dot.score(a, acc[o], it);
+                        k64 = make_key(v, (int32_t)(id0 + it));
+                        pass = v > -INFINITY && k64 > g.kth;
+                    }
+                    group_append(g, pass, k64);
+                }
+                group_check(g, a.k, a.train_indices, mlo, mhi);
+            }
         }
         if (tid == 0) n_cand = 0;
         __syncthreads();
@@ -377,45 +536,61 @@ __global__ __launch_bounds__(256) void pick_i8_kernel(MaxArgs m)
 }
 
 // ------------------------------------------------------------------------------------------
-// few items: a workgroup scores them all for one user, V per thread
+// few items: a workgroup scores them all for one user, 16 per thread at most
 // ------------------------------------------------------------------------------------------
-template <int V>
+template <int LPI>
 __global__ __launch_bounds__(256) void score_small_i8_kernel(ScoreI8Args a)
 {
+    constexpr int V = SMALL_ITEMS / 256;
     __shared__ GroupList g;
-    __shared__ uint32_t train[V * 256 / 32];
+    __shared__ uint32_t train[SMALL_ITEMS / 32];
     const int tid = threadIdx.x;
     const int64_t r = blockIdx.x;
     int32_t user;
     const int64_t prow = user_row(a, r, &user);
-    const int8_t *__restrict__ p = a.Pq + prow * a.ldp;
-    const float sp = a.sp[prow];
+    RowDot<LPI> dot;
+    dot.init(a, prow);
     const int64_t id0 = a.id_offset + a.item_lo;
-    for (int i = tid; i < V * 8; i += 256) train[i] = 0;
+    const int n_items = (int)a.n_items, own = RowDot<LPI>::owned();
+    for (int i = tid; i < SMALL_ITEMS / 32; i += 256) train[i] = 0;
     if (tid == 0) g.count = 0;
     __syncthreads();
     if (a.train_indptr)
         for (int64_t t = a.train_indptr[user] + tid, e = a.train_indptr[user + 1]; t < e; t += 256) {
             const int64_t i = a.train_indices[t] - id0;
-            if (i >= 0 && i < a.n_items) atomicOr(&train[i >> 5], 1u << (i & 31));
+            if (i >= 0 && i < n_items) atomicOr(&train[i >> 5], 1u << (i & 31));
         }
     __syncthreads();
     uint32_t key[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        const int i = 256 * v + tid;
         key[v] = 0;
-        if (i < a.n_items && !(train[i >> 5] >> (i & 31) & 1u)) {
-            const float s = score_item(a, p, sp, i);
+        if (256 * v >= n_items) continue;
+        uint4 q[LPI];
+#pragma unroll
+        for (int j = 0; j < LPI; ++j) {
+            const int i = 256 * v + j * (256 / LPI) + tid / LPI;
+            q[j] = dot.load(a, i < n_items ? i : 0);
+        }
+        int acc = 0;
+#pragma unroll
+        for (int j = 0; j < LPI; ++j) {
+            const int s = dot.dot(q[j]);
+            if (tid % LPI == j) acc = s;
+        }
+        const int i = 256 * v + own;
+        if (i < n_items && !(train[i >> 5] >> (i & 31) & 1u)) {
+            const float s = dot.score(a, acc, i);
             key[v] = s > -INFINITY ? f32_orderable(s) : 0u;
         }
     }
-    const uint32_t cut = rank_bound(key, a.k, g);
-    if (tid == 0) g.kth = ((uint64_t)cut << 32) - 1;
+    const uint32_t cut = rank_bound<256, V>(key, KEY_NONE, a.k, g);
+    if (tid == 0) g.kth = cut ? ((uint64_t)cut << 32) - 1 : ((uint64_t)KEY_NONE << 32 | 0xffffffffu);
     __syncthreads();
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        const uint64_t k64 = ((uint64_t)key[v] << 32) | (uint32_t)~(uint32_t)(id0 + 256 * v + tid);
+        if (256 * v >= n_items) continue;
+        const uint64_t k64 = ((uint64_t)key[v] << 32) | (uint32_t)~(uint32_t)(id0 + 256 * v + own);
         group_append(g, key[v] > KEY_NONE && k64 > g.kth, k64);
         group_check(g, a.k, nullptr, 0, 0);
     }
@@ -431,48 +606,82 @@ __global__ __launch_bounds__(256) void no_entries_kernel(int32_t *__restrict__ i
 // ------------------------------------------------------------------------------------------
 // host side
 // ------------------------------------------------------------------------------------------
-// users per pass of steps 1 and 2: their table of best scores stays below 512 MB (or holds 32 users)
-static int64_t users_per_pass(int64_t n, int64_t n_items)
+// users per pass of steps 1 and 2: their table of bounds stays below 512 MB (or holds 32 users)
+static int64_t users_per_pass(int64_t n, int64_t groups)
 {
-    const int64_t pitch = (n_items + 8 * BLOCK - 1) / (8 * BLOCK) * 8;
-    int64_t u = ((int64_t)512 << 20) / (pitch * 4) / 128 * 128;
+    int64_t u = ((int64_t)512 << 20) / (groups * 64) / 128 * 128;
     u = u < 32 ? 32 : u;
     return n < u ? n : u;
 }
 
-size_t tfrec_score_i8_bytes(int64_t n, int64_t n_items, int k)
+// sets of 32 users a wave of step 1 holds (registers: 4 for rows up to 128 bytes, 2 beyond)
+static int sets_per_wave(int64_t n, int d) { return n <= 32 ? 1 : (n <= 64 || d > 128 ? 2 : 4); }
+
+// slices of the items: enough waves for the chip (8 a CU), each with at least one group of 8 blocks
+static int split_items(int64_t n, int64_t groups, int d, int64_t *groups_per_split)
 {
-    if (n <= 0 || n_items <= SMALL_ITEMS) return 0;
-    const int64_t pitch = (n_items + 8 * BLOCK - 1) / (8 * BLOCK) * 8;
-    return tf_align((size_t)users_per_pass(n, n_items) * pitch * 4) + 512;
+    const int64_t user_groups = (n + 32 * sets_per_wave(n, d) - 1) / (32 * sets_per_wave(n, d));
+    int64_t splits = (2048 + user_groups - 1) / user_groups;
+    splits = splits < groups ? splits : groups;
+    *groups_per_split = (groups + splits - 1) / splits;
+    return (int)((groups + *groups_per_split - 1) / *groups_per_split);
 }
 
-static int launch_max(tfrec_ctx *ctx, MaxArgs m)
+static size_t slack_bytes(int64_t n, int64_t groups, int d)
 {
-    const ScoreI8Args &a = m.s;
+    // (a later, shorter pass has fewer user groups and so up to 2048 splits for its users)
+    return tf_align((size_t)4 * (n + 2048 * 32 * 4));
+}
+
+size_t tfrec_score_i8_bytes(int64_t n, int64_t n_items, int d, int k)
+{
+    if (n <= 0 || n_items <= SMALL_ITEMS) return 0;
+    const int64_t groups = (n_items + 8 * BLOCK - 1) / (8 * BLOCK), per_pass = users_per_pass(n, groups);
+    return tf_align((size_t)per_pass * groups * 64) + slack_bytes(per_pass, groups, d) + 512;
+}
+
+// calls f.operator()<LPI>() with the lanes an item's row takes
+template <class F>
+static int by_row_lanes(int d, F &&f)
+{
+    if (d <= 16) return f.template operator()<1>();
+    if (d <= 32) return f.template operator()<2>();
+    if (d <= 64) return f.template operator()<4>();
+    if (d <= 128) return f.template operator()<8>();
+    return f.template operator()<16>();
+}
+
+static int launch_max(tfrec_ctx *ctx, const MaxArgs &m)
+{
+    const int64_t grid = (int64_t)((m.splits + 7) / 8) * 8 * ((m.user_groups + 3) / 4);
+    TF_REQUIRE(grid < (1ll << 31), TFREC_EUNSUP, "too many users and items for one launch");
     auto go = [&]<int KS, int UW>() -> int {
-        m.user_groups = (int)((a.n + 32 * UW - 1) / (32 * UW));
-        const int wgs = (m.user_groups + 3) / 4;
-        // enough waves for the chip (8 a CU), each with at least one group of 8 blocks
-        int64_t splits = (2048 + m.user_groups - 1) / m.user_groups;
-        splits = splits < m.groups ? splits : m.groups;
-        m.groups_per_split = (m.groups + splits - 1) / splits;
-        m.splits = (int)((m.groups + m.groups_per_split - 1) / m.groups_per_split);
-        const int64_t grid = (int64_t)((m.splits + 7) / 8) * 8 * wgs;
-        TF_REQUIRE(grid < (1ll << 31), TFREC_EUNSUP, "too many users and items for one launch");
         score_max_i8_kernel<KS, UW><<<(unsigned)grid, 256, 0, ctx->stream>>>(m);
         TF_HIP(hipGetLastError());
         return TFREC_OK;
     };
+    const int uw = sets_per_wave(m.s.n, m.s.d);
     auto users = [&]<int KS>() -> int {
-        if (a.n <= 32) return go.template operator()<KS, 1>();
-        if (a.n <= 64 || KS == 8) return go.template operator()<KS, 2>();
-        return go.template operator()<KS, KS == 8 ? 2 : 4>();
+        if (uw == 1) return go.template operator()<KS, 1>();
+        if (uw == 2) return go.template operator()<KS, 2>();
+        if constexpr (KS <= 4) return go.template operator()<KS, 4>();
+        return TFREC_EUNSUP;       // (not reached: sets_per_wave)
     };
-    if (a.d <= 32) return users.template operator()<1>();
-    if (a.d <= 64) return users.template operator()<2>();
-    if (a.d <= 128) return users.template operator()<4>();
+    if (m.s.d <= 32) return users.template operator()<1>();
+    if (m.s.d <= 64) return users.template operator()<2>();
+    if (m.s.d <= 128) return users.template operator()<4>();
     return users.template operator()<8>();
+}
+
+static int launch_pick(tfrec_ctx *ctx, const MaxArgs &m)
+{
+    return by_row_lanes(m.s.d, [&]<int LPI>() -> int {
+        // few users leave most of the chip idle whatever their workgroups do: larger ones end sooner
+        if (m.s.n <= 256) pick_i8_kernel<1024, LPI><<<(unsigned)m.s.n, 1024, 0, ctx->stream>>>(m);
+        else pick_i8_kernel<256, LPI><<<(unsigned)m.s.n, 256, 0, ctx->stream>>>(m);
+        TF_HIP(hipGetLastError());
+        return TFREC_OK;
+    });
 }
 
 int tfrec_score_i8(tfrec_ctx *ctx, ScoreI8Args a)
@@ -484,24 +693,22 @@ int tfrec_score_i8(tfrec_ctx *ctx, ScoreI8Args a)
         return TFREC_OK;
     }
     a.flags = ctx->d_flags;
-    if (a.n_items <= SMALL_ITEMS) {
-        const unsigned n = (unsigned)a.n;
-        if (a.n_items <= 256) score_small_i8_kernel<1><<<n, 256, 0, ctx->stream>>>(a);
-        else if (a.n_items <= 512) score_small_i8_kernel<2><<<n, 256, 0, ctx->stream>>>(a);
-        else if (a.n_items <= 1024) score_small_i8_kernel<4><<<n, 256, 0, ctx->stream>>>(a);
-        else if (a.n_items <= 2048) score_small_i8_kernel<8><<<n, 256, 0, ctx->stream>>>(a);
-        else score_small_i8_kernel<16><<<n, 256, 0, ctx->stream>>>(a);
-        TF_HIP(hipGetLastError());
-        return TFREC_OK;
-    }
+    if (a.n_items <= SMALL_ITEMS)
+        return by_row_lanes(a.d, [&]<int LPI>() -> int {
+            score_small_i8_kernel<LPI><<<(unsigned)a.n, 256, 0, ctx->stream>>>(a);
+            TF_HIP(hipGetLastError());
+            return TFREC_OK;
+        });
     MaxArgs m{};
     m.groups = (a.n_items + 8 * BLOCK - 1) / (8 * BLOCK);
-    m.pitch = m.groups * 8;
-    const int64_t per_pass = users_per_pass(a.n, a.n_items);
-    TF_TRY(tfrec_ws_require(ctx, ctx->ws_used + tfrec_score_i8_bytes(a.n, a.n_items, a.k)));
+    m.pitch = m.groups * 16;
+    const int64_t per_pass = users_per_pass(a.n, m.groups);
+    TF_TRY(tfrec_ws_require(ctx, ctx->ws_used + tfrec_score_i8_bytes(a.n, a.n_items, a.d, a.k)));
     TF_TRY(tfrec_note_capture(ctx));
-    m.best = (float *)tfrec_ws_take(ctx, (size_t)per_pass * m.pitch * 4);
-    TF_REQUIRE(m.best != nullptr, TFREC_ENOMEM, "internal: workspace carve failed");
+    m.bound = (float *)tfrec_ws_take(ctx, (size_t)per_pass * m.pitch * 4);
+    const size_t slack = slack_bytes(per_pass, m.groups, a.d);
+    m.slack = (float *)tfrec_ws_take(ctx, slack);
+    TF_REQUIRE(m.bound != nullptr && m.slack != nullptr, TFREC_ENOMEM, "internal: workspace carve failed");
     for (int64_t u0 = 0; u0 < a.n; u0 += per_pass) {
         m.s = a;
         m.s.n = a.n - u0 < per_pass ? a.n - u0 : per_pass;
@@ -509,9 +716,12 @@ int tfrec_score_i8(tfrec_ctx *ctx, ScoreI8Args a)
         if (a.p_compact) { m.s.Pq = a.Pq + u0 * a.ldp; m.s.sp = a.sp + u0; }
         m.s.out_ids = a.out_ids + u0 * a.k;
         m.s.out_scores = a.out_scores + u0 * a.k;
+        m.splits = split_items(m.s.n, m.groups, a.d, &m.groups_per_split);
+        const int users = 32 * sets_per_wave(m.s.n, a.d);
+        m.user_groups = (int)((m.s.n + users - 1) / users);
+        TF_REQUIRE((size_t)m.s.n * m.splits * 4 <= slack, TFREC_ENOMEM, "internal: scratch too small");
         TF_TRY(launch_max(ctx, m));
-        pick_i8_kernel<<<(unsigned)m.s.n, 256, 0, ctx->stream>>>(m);
-        TF_HIP(hipGetLastError());
+        TF_TRY(launch_pick(ctx, m));
     }
     return TFREC_OK;
 }
