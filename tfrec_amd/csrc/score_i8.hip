@@ -20,7 +20,6 @@
 
 typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
 typedef int32_t i32x16 __attribute__((ext_vector_type(16)));
-struct __attribute__((packed, aligned(4))) Float4 { float v[4]; };       // 16 bytes at the alignment of a float
 
 static constexpr int BLOCK = 32, CELL = 16;    // items per block (a matrix instruction's rows) and per cell
 static constexpr int SMALL_ITEMS = 4096;       // (16 scores per thread of score_small_i8_kernel)
@@ -114,6 +113,7 @@ template <int KS, int UW>
 __global__ __launch_bounds__(256, 2) void score_max_i8_kernel(MaxArgs m)
 {
     __shared__ float out[4][UW][16][32];
+    __shared__ __align__(16) float scales[4][2][64];
     const ScoreI8Args &a = m.s;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 31, h = lane >> 5;
     // consecutive workgroups go to the 8 XCDs in turn: an XCD takes every 8th slice of the items, for all users one after
@@ -155,73 +155,88 @@ __global__ __launch_bounds__(256, 2) void score_max_i8_kernel(MaxArgs m)
     }
     const int8_t *__restrict__ Q = a.Qq + a.item_lo * a.ldq;
     const float *__restrict__ sq = a.sq + a.item_lo, *__restrict__ bias = a.b ? a.b + a.item_lo : nullptr;
-    struct Block { i32x4 q[KS]; Float4 sq[4], b[4]; };
+    // a block as this lane holds it before its turn: its chunks of row r, and (h = 0) the scale or (h = 1) the bias of item r
+    struct Block { i32x4 q[KS]; float sb; };
+    const float *__restrict__ sb_src = h && bias ? bias : sq;
     auto load = [&](Block &o, int64_t blk) {
-        const int64_t it = blk * BLOCK;
-        const int64_t row = it + r < a.n_items ? it + r : a.n_items - 1;
+        const int64_t i = blk * BLOCK + r, row = i < a.n_items ? i : a.n_items - 1;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) o.q[ks] = *reinterpret_cast<const i32x4 *>(Q + row * a.ldq + off[ks]);
-        if (it + BLOCK <= a.n_items) {
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                o.sq[g] = *reinterpret_cast<const Float4 *>(sq + it + 8 * g + 4 * h);
-                if (bias) o.b[g] = *reinterpret_cast<const Float4 *>(bias + it + 8 * g + 4 * h);
-                else o.b[g] = Float4{{0.f, 0.f, 0.f, 0.f}};
-            }
-        } else {
-            // the last block, or one past it: items that do not exist score -inf
-#pragma unroll
-            for (int g = 0; g < 4; ++g)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int64_t i = it + 8 * g + 4 * h + j;
-                    o.sq[g].v[j] = i < a.n_items ? sq[i] : 0.f;
-                    o.b[g].v[j] = i < a.n_items ? (bias ? bias[i] : 0.f) : -INFINITY;
-                }
-        }
+        o.sb = sb_src[row];
+        if (h && !bias) o.sb = 0.f;
+        if (i >= a.n_items) o.sb = h ? -INFINITY : 0.f;        // (past the last item: a score of -inf)
     };
     i32x16 start;
 #pragma unroll
     for (int e = 0; e < 16; ++e) start[e] = 0x4B400000;
-    Block cur;
-    load(cur, g0 * 8);
-    for (int64_t g = g0; g < g1; ++g) {
-#pragma unroll 1
-        for (int i = 0; i < 8; ++i) {
-            Block next;
-            load(next, g * 8 + i + 1);
-            float sqm = 0.f;
+    // kept in registers, not made again for every product, where there are registers for it
+    if constexpr (KS < 4) asm volatile("" : "+v"(start));
+    // long rows leave no registers to hold the next block's first products
+    constexpr bool AHEAD = KS < 8;
+    auto products = [&](const Block &o, int s) {
+        i32x16 acc = start;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) sqm = fmaxf(sqm, cur.sq[e >> 2].v[e & 3]);
-            const bool wide = __ballot(wide_user || sqm > 0x1p50f) != 0;
-            i32x16 acc[2];
-            acc[0] = start;
+        for (int ks = 0; ks < KS; ++ks) acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(o.q[ks], pb[s][ks], acc, 0, 0, 0);
+        return acc;
+    };
+    i32x16 acc;                // products of the set whose vector work comes next
+    auto step = [&](Block &cur, Block &next, int64_t g, int i) {
+        // the scales and biases of the lane's 16 items come through LDS: as loads from memory, eight of 16 bytes a lane for
+        // 2 * 16 values, they would keep the memory pipe as busy as the vector pipe
+        scales[wave][i & 1][lane] = cur.sb;
+        if constexpr (!AHEAD) acc = products(cur, 0);
+        load(next, g * 8 + i + 1);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        float sqv[16], bv[16];
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) acc[0] = __builtin_amdgcn_mfma_i32_32x32x32_i8(cur.q[ks], pb[0][ks], acc[0], 0, 0, 0);
+        for (int q = 0; q < 4; ++q) {
+            const float4 x = *reinterpret_cast<const float4 *>(&scales[wave][i & 1][8 * q + 4 * h]);
+            const float4 y = *reinterpret_cast<const float4 *>(&scales[wave][i & 1][32 + 8 * q + 4 * h]);
+            sqv[4 * q] = x.x; sqv[4 * q + 1] = x.y; sqv[4 * q + 2] = x.z; sqv[4 * q + 3] = x.w;
+            bv[4 * q] = y.x; bv[4 * q + 1] = y.y; bv[4 * q + 2] = y.z; bv[4 * q + 3] = y.w;
+        }
+        float sqm = 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sqm = fmaxf(sqm, sqv[e]);
+        auto keep = [&](int s, float mx, float d) {
+            slack[s] = fmaxf(slack[s], d);
+            out[wave][s][2 * i + h][r] = mx + fmaf(fabsf(mx), 0x1p-21f, d);
+        };
+        // the products of the next set (after the last, of the next block's first) are issued before the vector work on this
+        // set's, and the matrix pipe has them done when their turn comes
+        auto sets = [&]<bool PLAIN>() {
 #pragma unroll
             for (int s = 0; s < UW; ++s) {
-                // the next set's products run beside this set's vector work
-                if (s + 1 < UW) {
-                    acc[(s + 1) & 1] = start;
+                const i32x16 x = acc;
+                __builtin_amdgcn_sched_barrier(0);
+                if (s + 1 < UW) acc = products(cur, s + 1);
+                else if constexpr (AHEAD) acc = products(next, 0);
+                __builtin_amdgcn_sched_barrier(0);
+                float mx = LOWEST;
+                if constexpr (PLAIN) {
 #pragma unroll
-                    for (int ks = 0; ks < KS; ++ks) acc[(s + 1) & 1] = __builtin_amdgcn_mfma_i32_32x32x32_i8(cur.q[ks], pb[s + 1][ks], acc[(s + 1) & 1], 0, 0, 0);
-                }
-                const i32x16 &x = acc[s & 1];
-                float mx = LOWEST, d = 0x1p-140f;
-                if (!wide) {
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) mx = fmaxf(mx, fmaf(fmaf(__int_as_float(x[e]), sp[s], off_sp[s]), cur.sq[e >> 2].v[e & 3], cur.b[e >> 2].v[e & 3]));
-                    d = fmaf(err_sp[s], sqm, d);
+                    for (int e = 0; e < 16; ++e) mx = fmaxf(mx, fmaf(fmaf(__int_as_float(x[e]), sp[s], off_sp[s]), sqv[e], bv[e]));
+                    keep(s, mx, fmaf(err_sp[s], sqm, 0x1p-140f));
                 } else {
 #pragma unroll
                     for (int e = 0; e < 16; ++e)
-                        mx = fmaxf(mx, add_rounded(scaled_sum(x[e] - 0x4B400000, sp[s], cur.sq[e >> 2].v[e & 3]), cur.b[e >> 2].v[e & 3]));
+                        mx = fmaxf(mx, add_rounded(scaled_sum(x[e] - 0x4B400000, sp[s], sqv[e]), bv[e]));
+                    keep(s, mx, 0x1p-140f);
                 }
-                slack[s] = fmaxf(slack[s], d);
-                d = fmaf(fabsf(mx), 0x1p-21f, d);
-                out[wave][s][2 * i + h][r] = mx + d;
             }
-            cur = next;
+        };
+        if (__ballot(wide_user || sqm > 0x1p50f) == 0) [[likely]] sets.template operator()<true>();
+        else sets.template operator()<false>();
+    };
+    Block even, odd;
+    load(even, g0 * 8);
+    if (AHEAD) acc = products(even, 0);
+    for (int64_t g = g0; g < g1; ++g) {
+#pragma unroll 1
+        for (int i = 0; i < 8; i += 2) {
+            step(even, odd, g, i);
+            step(odd, even, g, i + 1);
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -251,7 +266,10 @@ __global__ __launch_bounds__(256, 2) void score_max_i8_kernel(MaxArgs m)
 // ------------------------------------------------------------------------------------------
 // a workgroup's list of keys (scored by 256 threads; NT threads in all)
 // ------------------------------------------------------------------------------------------
-static constexpr int LIST = 1024;
+// LIST keys at most: room for k and for the 256 that one step may add.  512 up to k = 112 (a quarter of the registers and
+// half the LDS of 1024, which is what bounds the workgroups a CU holds: 110 -> see pick_i8_kernel), else 1024.
+static inline int list_for(int k) { return k <= 112 ? 512 : 1024; }
+template <int LIST>
 struct GroupList {
     uint64_t list[LIST], sorted[LIST];
     uint64_t kth;              // keys at or below it are not wanted
@@ -264,8 +282,8 @@ struct GroupList {
 // A lower bound of the k-th largest of the workgroup's orderable values (V per thread; values at or below `none` are
 // none): the lower edge of a bucket of a two-level histogram below the highest bit in which the values differ.
 // 0 if fewer than k values are held.
-template <int NT, int V>
-__device__ __forceinline__ uint32_t rank_bound(const uint32_t (&key)[V], uint32_t none, int k, GroupList &g)
+template <int NT, int V, class List>
+__device__ __forceinline__ uint32_t rank_bound(const uint32_t (&key)[V], uint32_t none, int k, List &g)
 {
     constexpr int NW = NT / 64;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -330,7 +348,8 @@ __device__ __forceinline__ uint32_t rank_bound(const uint32_t (&key)[V], uint32_
 }
 
 // a wave's keys that pass go to the list; all lanes call it
-__device__ __forceinline__ void group_append(GroupList &g, bool pass, uint64_t key)
+template <class List>
+__device__ __forceinline__ void group_append(List &g, bool pass, uint64_t key)
 {
     const int lane = threadIdx.x & 63;
     const uint64_t m = __ballot(pass);
@@ -343,7 +362,8 @@ __device__ __forceinline__ void group_append(GroupList &g, bool pass, uint64_t k
 
 // called by all threads after a step that appended at most 256 keys: cuts the list back to its k best once the next step might
 // not fit
-__device__ __forceinline__ void group_check(GroupList &g, int k, const int32_t *midx, int64_t mlo, int64_t mhi)
+template <int LIST>
+__device__ __forceinline__ void group_check(GroupList<LIST> &g, int k, const int32_t *midx, int64_t mlo, int64_t mhi)
 {
     __syncthreads();
     if (g.count > LIST - 256) {
@@ -360,7 +380,8 @@ __device__ __forceinline__ void group_check(GroupList &g, int k, const int32_t *
 }
 
 // the list's k best in order, by the first wave
-__device__ __forceinline__ void group_finish(GroupList &g, const ScoreI8Args &a, int64_t r, const int32_t *midx, int64_t mlo, int64_t mhi)
+template <int LIST>
+__device__ __forceinline__ void group_finish(GroupList<LIST> &g, const ScoreI8Args &a, int64_t r, const int32_t *midx, int64_t mlo, int64_t mhi)
 {
     __syncthreads();
     if (threadIdx.x >= 64) return;
@@ -380,17 +401,17 @@ __device__ __forceinline__ void group_finish(GroupList &g, const ScoreI8Args &a,
 // step 2: the cells that can hold a listed item, scored again
 // ------------------------------------------------------------------------------------------
 static constexpr int SLICES = 1024;            // groups of cells: cell y belongs to slice y % SLICES
-static constexpr int CAND = 2048;              // cells per round
+static constexpr int CAND = 1024;              // cells per round
 
 // first item of cell y, and item e of it
 __device__ __forceinline__ int64_t cell_first(int64_t y) { return (y >> 1) * BLOCK + 4 * (y & 1); }
 __device__ __forceinline__ int64_t cell_item(int64_t y, int e) { return cell_first(y) + 8 * (e >> 2) + (e & 3); }
 
 // NT = 256 threads, or 1024 where there are few users and one workgroup's time is the call's; LPI: see RowDot
-template <int NT, int LPI>
+template <int NT, int LPI, int LIST>
 __global__ __launch_bounds__(NT) void pick_i8_kernel(MaxArgs m)
 {
-    __shared__ GroupList g;
+    __shared__ GroupList<LIST> g;
     __shared__ uint32_t cand[CAND];
     __shared__ uint16_t slices[SLICES];
     __shared__ uint8_t train[SLICES];
@@ -538,11 +559,11 @@ __global__ __launch_bounds__(NT) void pick_i8_kernel(MaxArgs m)
 // ------------------------------------------------------------------------------------------
 // few items: a workgroup scores them all for one user, 16 per thread at most
 // ------------------------------------------------------------------------------------------
-template <int LPI>
+template <int LPI, int LIST>
 __global__ __launch_bounds__(256) void score_small_i8_kernel(ScoreI8Args a)
 {
     constexpr int V = SMALL_ITEMS / 256;
-    __shared__ GroupList g;
+    __shared__ GroupList<LIST> g;
     __shared__ uint32_t train[SMALL_ITEMS / 32];
     const int tid = threadIdx.x;
     const int64_t r = blockIdx.x;
@@ -614,8 +635,9 @@ static int64_t users_per_pass(int64_t n, int64_t groups)
     return n < u ? n : u;
 }
 
-// sets of 32 users a wave of step 1 holds (registers: 4 for rows up to 128 bytes, 2 beyond)
-static int sets_per_wave(int64_t n, int d) { return n <= 32 ? 1 : (n <= 64 || d > 128 ? 2 : 4); }
+// sets of 32 users a wave of step 1 holds: as many as its 256 registers take beside two blocks of items (4 for rows of up to
+// 64 bytes, 3 up to 128, 2 beyond)
+static int sets_per_wave(int64_t n, int d) { return n <= 32 ? 1 : (n <= 64 || d > 128 ? 2 : (d > 64 ? 3 : 4)); }
 
 // slices of the items: enough waves for the chip (8 a CU), each with at least one group of 8 blocks
 static int split_items(int64_t n, int64_t groups, int d, int64_t *groups_per_split)
@@ -664,8 +686,7 @@ static int launch_max(tfrec_ctx *ctx, const MaxArgs &m)
     auto users = [&]<int KS>() -> int {
         if (uw == 1) return go.template operator()<KS, 1>();
         if (uw == 2) return go.template operator()<KS, 2>();
-        if constexpr (KS <= 4) return go.template operator()<KS, 4>();
-        return TFREC_EUNSUP;       // (not reached: sets_per_wave)
+        return go.template operator()<KS, KS <= 2 ? 4 : (KS == 4 ? 3 : 2)>();
     };
     if (m.s.d <= 32) return users.template operator()<1>();
     if (m.s.d <= 64) return users.template operator()<2>();
@@ -677,8 +698,14 @@ static int launch_pick(tfrec_ctx *ctx, const MaxArgs &m)
 {
     return by_row_lanes(m.s.d, [&]<int LPI>() -> int {
         // few users leave most of the chip idle whatever their workgroups do: larger ones end sooner
-        if (m.s.n <= 256) pick_i8_kernel<1024, LPI><<<(unsigned)m.s.n, 1024, 0, ctx->stream>>>(m);
-        else pick_i8_kernel<256, LPI><<<(unsigned)m.s.n, 256, 0, ctx->stream>>>(m);
+        const unsigned n = (unsigned)m.s.n;
+        if (list_for(m.s.k) == 512) {
+            if (n <= 256) pick_i8_kernel<1024, LPI, 512><<<n, 1024, 0, ctx->stream>>>(m);
+            else pick_i8_kernel<256, LPI, 512><<<n, 256, 0, ctx->stream>>>(m);
+        } else {
+            if (n <= 256) pick_i8_kernel<1024, LPI, 1024><<<n, 1024, 0, ctx->stream>>>(m);
+            else pick_i8_kernel<256, LPI, 1024><<<n, 256, 0, ctx->stream>>>(m);
+        }
         TF_HIP(hipGetLastError());
         return TFREC_OK;
     });
@@ -695,7 +722,8 @@ int tfrec_score_i8(tfrec_ctx *ctx, ScoreI8Args a)
     a.flags = ctx->d_flags;
     if (a.n_items <= SMALL_ITEMS)
         return by_row_lanes(a.d, [&]<int LPI>() -> int {
-            score_small_i8_kernel<LPI><<<(unsigned)a.n, 256, 0, ctx->stream>>>(a);
+            if (list_for(a.k) == 512) score_small_i8_kernel<LPI, 512><<<(unsigned)a.n, 256, 0, ctx->stream>>>(a);
+            else score_small_i8_kernel<LPI, 1024><<<(unsigned)a.n, 256, 0, ctx->stream>>>(a);
             TF_HIP(hipGetLastError());
             return TFREC_OK;
         });
