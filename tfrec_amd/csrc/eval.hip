@@ -1002,7 +1002,7 @@ static int cap_for(int k, bool bf16, int D)
 
 // the dynamic-LDS limit is a per-device attribute of a kernel: set once on every device an instantiation runs on
 // (bit = device ordinal; devices beyond 63 set it on every launch)
-static int raise_lds_limit(tfrec_ctx *ctx, const void *kernel, int bytes, std::atomic<uint64_t> &done)
+int tfrec_raise_lds_limit(tfrec_ctx *ctx, const void *kernel, int bytes, std::atomic<uint64_t> &done)
 {
     const uint64_t dev_bit = ctx->device < 64 ? (1ull << ctx->device) : 0ull;
     if (!(done.load(std::memory_order_acquire) & dev_bit)) {
@@ -1017,7 +1017,7 @@ static int launch_score_pp(tfrec_ctx *ctx, const ScoreArgs &a, int splits)
 {
     using G = PpGeom<D, CAP>;
     static std::atomic<uint64_t> attr_devices{0};
-    TF_TRY(raise_lds_limit(ctx, reinterpret_cast<const void *>(&score_topk_pp_kernel<D, CAP>), G::LDS_BYTES, attr_devices));
+    TF_TRY(tfrec_raise_lds_limit(ctx, reinterpret_cast<const void *>(&score_topk_pp_kernel<D, CAP>), G::LDS_BYTES, attr_devices));
     const int user_blocks = (int)((a.n + G::UB - 1) / G::UB);
     score_topk_pp_kernel<D, CAP><<<dim3(user_blocks, splits), G::NT, G::LDS_BYTES, ctx->stream>>>(a);
     TF_HIP(hipGetLastError());
@@ -1035,7 +1035,7 @@ static int launch_score(tfrec_ctx *ctx, const ScoreArgs &a, int user_blocks, int
     }
     using G = ScoreGeom<D, BF16, CAP>;
     static std::atomic<uint64_t> attr_devices{0};
-    TF_TRY(raise_lds_limit(ctx, reinterpret_cast<const void *>(&score_topk_kernel<D, BF16, CAP>), G::LDS_BYTES, attr_devices));
+    TF_TRY(tfrec_raise_lds_limit(ctx, reinterpret_cast<const void *>(&score_topk_kernel<D, BF16, CAP>), G::LDS_BYTES, attr_devices));
     // the caller counts workgroups of 128 users; this instantiation may hold more
     constexpr int UB = 32 * G::NW * ScoreWave<D, BF16, CAP>::UW;
     user_blocks = (int)((a.n + UB - 1) / UB);

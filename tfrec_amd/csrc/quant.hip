@@ -2,6 +2,8 @@
 #include "i8_device.hpp"
 #include "score_i8.hpp"
 
+#include <atomic>
+
 typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
 typedef int32_t i32x16 __attribute__((ext_vector_type(16)));
 
@@ -24,23 +26,24 @@ __device__ __forceinline__ int quantize_one(float x, float s, float inv)
     return (int)fminf(fmaxf(r, -127.f), 127.f);
 }
 
+// 16 values at the alignment of their type (global memory takes 16-byte accesses at any)
 template <class T>
-struct Elem;
-template <> struct Elem<float> { static __device__ __forceinline__ float get(const float *p) { return *p; } };
-template <> struct Elem<__bf16> { static __device__ __forceinline__ float get(const __bf16 *p) { return (float)*p; } };
-template <> struct Elem<_Float16> { static __device__ __forceinline__ float get(const _Float16 *p) { return (float)*p; } };
+struct __attribute__((packed, aligned(sizeof(T)))) Values16 { T v[16]; };
 
-// LPR lanes (a power of two up to 64) hold one row, 16 columns per lane and round; two rounds over the row (the second
-// finds it in the caches).
-template <class T, int LPR>
+// LPR threads hold one row (a power of two up to 64: lanes of a wave; 256: the workgroup), CH runs of 16 columns each in
+// registers: one read of the row, one write of a quarter (half) as much.  CH = 0: rows too long for that are read twice,
+// the second time from the caches.
+// Bound by memory: 4096 x 8192 bf16 (96 MB in all) in the time the launch code below gives.
+template <class T, int LPR, int CH>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(const T *__restrict__ X, int64_t n_rows, int64_t ldx, int64_t d,
                                                             const int32_t *__restrict__ rows, int64_t n, int8_t *__restrict__ q, int64_t ldq,
                                                             float *__restrict__ scale, uint32_t *__restrict__ flags)
 {
     constexpr int GPB = 256 / LPR;
     const int gl = threadIdx.x % LPR;
-    const int64_t r = (int64_t)blockIdx.x * GPB + threadIdx.x / LPR;
-    if (r >= n) return;
+    int64_t r = (int64_t)blockIdx.x * GPB + threadIdx.x / LPR;
+    const bool live = r < n;                   // (threads past the last row stay for the workgroup's barrier)
+    r = live ? r : n - 1;
     int64_t src = r;
     if (rows) {
         const int32_t id = rows[r];
@@ -49,31 +52,61 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const T *__restrict_
     }
     const T *x = X + src * ldx;
     const int64_t chunks = (d + 15) / 16;
+    auto load = [&](int64_t c) {
+        Values16<T> v;
+        if (c * 16 + 16 <= d) v = *reinterpret_cast<const Values16<T> *>(x + c * 16);
+        else
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v.v[j] = c * 16 + j < d ? x[c * 16 + j] : (T)0.f;
+        return v;
+    };
     float mx = 0.f;
     bool bad = false;
-    for (int64_t c = gl; c < chunks; c += LPR)
-        for (int j = 0; j < 16; ++j)
-            if (c * 16 + j < d) {
-                const float v = fabsf(Elem<T>::get(x + c * 16 + j));
-                bad |= !(v < INFINITY);
-                mx = fmaxf(mx, v);
-            }
+    auto look = [&](const Values16<T> &v) {
 #pragma unroll
-    for (int off = LPR / 2; off > 0; off >>= 1) {
-        mx = fmaxf(mx, __shfl_xor(mx, off, 64));
-        bad |= __shfl_xor((int)bad, off, 64) != 0;
+        for (int j = 0; j < 16; ++j) {
+            const float f = fabsf((float)v.v[j]);
+            bad |= !(f < INFINITY);
+            mx = fmaxf(mx, f);
+        }
+    };
+    Values16<T> held[CH > 0 ? CH : 1];
+    if constexpr (CH > 0) {
+#pragma unroll
+        for (int i = 0; i < CH; ++i) held[i] = load(gl + i * LPR);          // (past the row: zeros)
+#pragma unroll
+        for (int i = 0; i < CH; ++i) look(held[i]);
+    } else {
+        for (int64_t c = gl; c < chunks; c += LPR) look(load(c));
     }
+    mx = bad ? INFINITY : mx;
+#pragma unroll
+    for (int off = (LPR < 64 ? LPR : 64) / 2; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off, 64));
+    if constexpr (LPR > 64) {
+        __shared__ float part[4];
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = mx;
+        __syncthreads();
+        mx = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+    }
+    if (!live) return;
     float s = mx / 127.0f;
-    if (gl == 0) scale[r] = bad ? NAN : s;
-    const bool none = bad || !(s > 0.f);
+    const bool none = !(mx < INFINITY) || !(s > 0.f);
+    if (gl == 0) scale[r] = mx < INFINITY ? s : NAN;
     const float up = s < 0x1p-60f ? 0x1p64f : 1.f;
     s *= up;
     const float inv = 1.f / s;
-    for (int64_t c = gl; c < chunks; c += LPR) {
+    auto put = [&](int64_t c, const Values16<T> &v) {
         union { int8_t b[16]; uint4 v; } o;
-        for (int j = 0; j < 16; ++j)
-            o.b[j] = !none && c * 16 + j < d ? (int8_t)quantize_one(Elem<T>::get(x + c * 16 + j) * up, s, inv) : 0;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o.b[j] = none ? 0 : (int8_t)quantize_one((float)v.v[j] * up, s, inv);
         *reinterpret_cast<uint4 *>(q + r * ldq + c * 16) = o.v;
+    };
+    if constexpr (CH > 0) {
+#pragma unroll
+        for (int i = 0; i < CH; ++i)
+            if (gl + i * LPR < chunks) put(gl + i * LPR, held[i]);
+    } else {
+        for (int64_t c = gl; c < chunks; c += LPR) put(c, load(c));
     }
 }
 
@@ -81,18 +114,21 @@ template <class T>
 static int launch_quantize(tfrec_ctx *ctx, const void *X, int64_t n_rows, int64_t ldx, int64_t d, const int32_t *rows, int64_t n, int8_t *q,
                            int64_t ldq, float *scale)
 {
-    auto go = [&]<int LPR>() -> int {
+    auto go = [&]<int LPR, int CH>() -> int {
         constexpr int GPB = 256 / LPR;
         const int64_t blocks = (n + GPB - 1) / GPB;
         TF_REQUIRE(blocks < (1ll << 31), TFREC_EUNSUP, "too many rows");
-        quantize_rows_kernel<T, LPR><<<(unsigned)blocks, 256, 0, ctx->stream>>>((const T *)X, n_rows, ldx, d, rows, n, q, ldq, scale, ctx->d_flags);
+        quantize_rows_kernel<T, LPR, CH><<<(unsigned)blocks, 256, 0, ctx->stream>>>((const T *)X, n_rows, ldx, d, rows, n, q, ldq, scale, ctx->d_flags);
         TF_HIP(hipGetLastError());
         return TFREC_OK;
     };
     const int64_t chunks = (d + 15) / 16;
-    if (chunks <= 4) return go.template operator()<4>();
-    if (chunks <= 16) return go.template operator()<16>();
-    return go.template operator()<64>();
+    if (chunks <= 4) return go.template operator()<4, 1>();
+    if (chunks <= 16) return go.template operator()<16, 1>();
+    if (chunks <= 64) return go.template operator()<64, 1>();
+    if (chunks <= 256) return go.template operator()<256, 1>();
+    if (chunks <= 512) return go.template operator()<256, 2>();
+    return go.template operator()<256, 0>();
 }
 
 int tfrec_quantize_rows(tfrec_ctx *ctx, const void *d_X, int x_dtype, int64_t n_rows, int64_t ldx, int64_t d, const int32_t *d_rows, int64_t n,
@@ -139,8 +175,99 @@ struct MatmulArgs {
     int64_t lda, ldb, ldc, M, N, K;
 };
 
-template <class T>
-__device__ __forceinline__ void store_out(void *C, int64_t at, float v) { reinterpret_cast<T *>(C)[at] = (T)v; }
+// one value of C before it is rounded to C's type
+__device__ __forceinline__ float output(const MatmulArgs &a, int acc, float sa, float sb, float bias)
+{
+    const float v = scaled_sum(acc, sa, sb);
+    return a.bias ? add_rounded(v, bias) : v;
+}
+
+// ---- few rows of A, or few tiles: 16 rows of B by 16 MT rows of A per workgroup, its KW waves sharing K ----------------
+// Bound by reading B (one row of A) or by latency (small products): B's rows come straight from memory as the matrix
+// instruction's A operand (16 x 16 x 64: lane l holds 16 bytes of row l & 15, columns 16 (l >> 4) .. + 16; result register
+// j is row 4 (l >> 4) + j, column l & 15), all of a wave's loads of several steps in flight, and the waves' whole-number sums
+// are added in LDS.
+template <class T, int MT, int KW>
+__global__ __launch_bounds__(64 * KW) void matmul_i8_rows_kernel(MatmulArgs a)
+{
+    __shared__ int32_t part[KW > 1 ? KW - 1 : 1][MT][4][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, c16 = (lane >> 4) * 16;
+    const int64_t n0 = (int64_t)blockIdx.x * 16, m0 = (int64_t)blockIdx.y * (16 * MT);
+    const int8_t *bp = a.B + (n0 + r < a.N ? n0 + r : a.N - 1) * a.ldb;
+    const int8_t *ap[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+        const int64_t m = m0 + 16 * t + r;
+        ap[t] = a.A + (m < a.M ? m : a.M - 1) * a.lda;
+    }
+    i32x4 acc[MT] = {};
+    // steps of 64 columns; wave w takes steps w, w + KW, ...
+    const int steps = (int)(a.K / 64);
+    constexpr int DEPTH = MT <= 2 ? 4 : (MT == 4 ? 2 : 1);
+    int s = wave;
+    for (; s + (DEPTH - 1) * KW < steps; s += DEPTH * KW) {
+        i32x4 fb[DEPTH], fa[DEPTH][MT];
+#pragma unroll
+        for (int q = 0; q < DEPTH; ++q) {
+            const int64_t k = (int64_t)(s + q * KW) * 64 + c16;
+            fb[q] = *reinterpret_cast<const i32x4 *>(bp + k);
+#pragma unroll
+            for (int t = 0; t < MT; ++t) fa[q][t] = *reinterpret_cast<const i32x4 *>(ap[t] + k);
+        }
+#pragma unroll
+        for (int q = 0; q < DEPTH; ++q)
+#pragma unroll
+            for (int t = 0; t < MT; ++t) acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fb[q], fa[q][t], acc[t], 0, 0, 0);
+    }
+    for (; s * 64 < a.K; s += KW) {
+        // what is left, up to a last step that ends inside 64 columns: A is zero there, B any bytes of its row
+        const int64_t k = (int64_t)s * 64 + c16;
+        const i32x4 fb = *reinterpret_cast<const i32x4 *>(bp + (k < a.K ? k : 0));
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (k < a.K) v = keep_below(*reinterpret_cast<const uint4 *>(ap[t] + k), k, a.K);
+            acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fb, __builtin_bit_cast(i32x4, v), acc[t], 0, 0, 0);
+        }
+    }
+    if constexpr (KW > 1) {
+        if (wave > 0)
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) part[wave - 1][t][j][lane] = acc[t][j];
+        __syncthreads();
+        if (wave > 0) return;
+#pragma unroll
+        for (int w = 0; w < KW - 1; ++w)
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[t][j] += part[w][t][j][lane];
+    }
+    const int64_t n = n0 + (lane >> 4) * 4;
+    float sb[4], bias[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int64_t nj = n + j < a.N ? n + j : a.N - 1;
+        sb[j] = a.sb[nj];
+        bias[j] = a.bias ? a.bias[nj] : 0.f;
+    }
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+        const int64_t m = m0 + 16 * t + r;
+        if (m >= a.M) continue;
+        const float sa = a.sa[m];
+        T *to = reinterpret_cast<T *>(a.C) + m * a.ldc + n;
+        struct __attribute__((packed, aligned(sizeof(T)))) Four { T v[4]; } o;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o.v[j] = (T)output(a, acc[t][j], sa, sb[j], bias[j]);
+        if (n + 4 <= a.N) *reinterpret_cast<Four *>(to) = o;
+        else
+            for (int j = 0; j < 4; ++j)
+                if (n + j < a.N) to[j] = o.v[j];
+    }
+}
 
 // 128 x 128 of C per workgroup, 64 x 64 per wave in four 32 x 32 blocks of v_mfma_i32_32x32x32_i8.  Tiles of 64 columns go
 // through LDS (two buffers; rows of 64 bytes, the chunk position XORed with the row so that fragment reads spread over
@@ -214,20 +341,172 @@ __global__ __launch_bounds__(256) void matmul_i8_kernel(MatmulArgs a)
             for (int e = 0; e < 16; ++e) {
                 const int64_t m = m0 + wm + 32 * i + (e & 3) + 8 * (e >> 2) + 4 * h;
                 if (m < a.M) {
-                    float v = scaled_sum(acc[i][j][e], a.sa[m], sb);
-                    if (a.bias) v = add_rounded(v, bias);
-                    store_out<T>(a.C, m * a.ldc + n, v);
+                    reinterpret_cast<T *>(a.C)[m * a.ldc + n] = (T)output(a, acc[i][j][e], a.sa[m], sb, bias);
                 }
             }
     }
 }
 
+// ---- large products: 256 x 256 of C per workgroup of eight waves, 128 x 64 per wave ------------------------------------
+// Bound by the matrix cores.  A step takes 128 columns: 32 matrix instructions of 32 x 32 x 32 a wave, two waves a SIMD.
+// Rows go from memory straight into LDS (global_load_lds_dwordx4: one kilobyte, eight rows, per instruction and wave), two
+// buffers of 64 KB: the next step's loads are issued among this step's products.  The LDS image has no row padding; position
+// c of row r holds the row's chunk c ^ (r & 7), so that fragment reads spread over the banks (the swizzle is on the source
+// address).  Rows past the ends of A and B read the last row, columns past K are masked out of A's fragments in the last
+// step.  C goes out through LDS, so that stores cover whole 128-byte pieces of its rows.
+template <class T>
+using global_ptr = __attribute__((address_space(1))) T *;
+
+static constexpr int BIG_LDS = 131072 + 1024;      // two buffers, and A's 256 scales
+
+template <class T>
+__global__ __launch_bounds__(512) void matmul_i8_big_kernel(MatmulArgs a, int tiles_m, int tiles_n)
+{
+    constexpr int KB = 128, HALF = 256 * KB, BUF = 2 * HALF;
+    extern __shared__ __align__(16) char lds[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 31, h = lane >> 5;
+    // consecutive workgroups go to the 8 XCDs in turn: each XCD takes one run of tiles, four tiles of A rows at a time, so
+    // that the tiles it works on together share rows of A and B in its L2
+    const int tiles = tiles_m * tiles_n, per = (tiles + 7) / 8;
+    const int t = (int)(blockIdx.x % 8) * per + (int)(blockIdx.x / 8);
+    if (t >= tiles || (int)(blockIdx.x / 8) >= per) return;
+    const int band = t / (4 * tiles_n), in_band = t - band * 4 * tiles_n;
+    const int band_m = tiles_m - 4 * band < 4 ? tiles_m - 4 * band : 4;
+    const int64_t m0 = (int64_t)(4 * band + in_band % band_m) * 256, n0 = (int64_t)(in_band / band_m) * 256;
+
+    // this wave's rows of a step: 8 * (8 i + wave) + lane / 8 of A and of B, i = 0..3
+    const int chunk = ((lane & 7) ^ (lane >> 3)) * 16;
+    global_ptr<const char> src[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int64_t row = 8 * (8 * i + wave) + (lane >> 3);
+        src[i] = (global_ptr<const char>)(const char *)(a.A + (m0 + row < a.M ? m0 + row : a.M - 1) * a.lda);
+        src[4 + i] = (global_ptr<const char>)(const char *)(a.B + (n0 + row < a.N ? n0 + row : a.N - 1) * a.ldb);
+    }
+    float *scale_a = reinterpret_cast<float *>(lds + 2 * BUF);
+    if (tid < 256) scale_a[tid] = a.sa[m0 + tid < a.M ? m0 + tid : a.M - 1];
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
+    auto request = [&](int64_t k0, int buf, int i) {
+        const int64_t k = k0 + chunk;
+        const global_ptr<const char> from = src[i] + (k < a.K ? k : 0);
+        const uint32_t to = __builtin_amdgcn_readfirstlane(lds0 + (uint32_t)(buf * BUF + (i >> 2) * HALF + (8 * (i & 3) + wave) * 1024));
+        asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(to) : "memory", "m0");
+    };
+    const int wm = (wave >> 2) * 128, wn = (wave & 3) * 64;
+    int off[KB / 32];
+#pragma unroll
+    for (int ks = 0; ks < KB / 32; ++ks) off[ks] = r * KB + (((2 * ks + h) ^ (r & 7)) * 16);
+    i32x16 acc[4][2] = {};
+    const int64_t steps = (a.K + KB - 1) / KB;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) request(0, 0, i);
+    for (int64_t s = 0; s < steps; ++s) {
+        const int buf = (int)(s & 1);
+        const bool last = s + 1 == steps;
+        // this wave's loads of the step have landed, and after the barrier everyone's; everyone is also done with the other buffer
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        const char *A = lds + buf * BUF + wm * KB, *B = lds + buf * BUF + HALF + wn * KB;
+        i32x4 fa[2][4], fb[2][2];
+        auto fragments = [&](int ks, int to) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) fa[to][i] = *reinterpret_cast<const i32x4 *>(A + off[ks] + 32 * i * KB);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) fb[to][j] = *reinterpret_cast<const i32x4 *>(B + off[ks] + 32 * j * KB);
+            if (last)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) fa[to][i] = __builtin_bit_cast(i32x4, keep_below(__builtin_bit_cast(uint4, fa[to][i]), s * KB + 32 * ks + 16 * h, a.K));
+        };
+        fragments(0, 0);
+#pragma unroll
+        for (int ks = 0; ks < KB / 32; ++ks) {
+            if (ks + 1 < KB / 32) fragments(ks + 1, (ks + 1) & 1);
+            if (!last) {
+                request((s + 1) * KB, buf ^ 1, 2 * ks);
+                request((s + 1) * KB, buf ^ 1, 2 * ks + 1);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa[ks & 1][i], fb[ks & 1][j], acc[i][j], 0, 0, 0);
+        }
+    }
+    __syncthreads();
+
+    // C: a wave's 128 x 64 in pieces of 32 rows through its 16 KB of LDS (rows padded by 16 bytes)
+    constexpr int PITCH = 64 * sizeof(T) + 16, LANES = 64 * sizeof(T) / 16, PER = 16 / sizeof(T);
+    static_assert(32 * PITCH <= 16384, "a wave's piece exceeds its LDS");
+    char *mine = lds + wave * 16384;
+    float sb[2], bias[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int64_t n = n0 + wn + 32 * j + r, nc = n < a.N ? n : a.N - 1;
+        sb[j] = a.sb[nc];
+        bias[j] = a.bias ? a.bias[nc] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const int row = (e & 3) + 8 * (e >> 2) + 4 * h;
+            const float sa = scale_a[wm + 32 * i + row];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) *reinterpret_cast<T *>(mine + row * PITCH + (32 * j + r) * sizeof(T)) = (T)output(a, acc[i][j][e], sa, sb[j], bias[j]);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        struct __attribute__((packed, aligned(sizeof(T)))) Piece { T v[PER]; };
+#pragma unroll
+        for (int q = 0; q < 32 * LANES / 64; ++q) {
+            const int row = (64 * q + lane) / LANES, col = (64 * q + lane) % LANES * PER;
+            const int64_t m = m0 + wm + 32 * i + row, n = n0 + wn + col;
+            const uint4 v = *reinterpret_cast<const uint4 *>(mine + row * PITCH + col * sizeof(T));
+            if (m < a.M) {
+                T *to = reinterpret_cast<T *>(a.C) + m * a.ldc + n;
+                const Piece p = __builtin_bit_cast(Piece, v);
+                if (n + PER <= a.N) *reinterpret_cast<Piece *>(to) = p;
+                else
+                    for (int x = 0; x < PER; ++x)
+                        if (n + x < a.N) to[x] = p.v[x];
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+
+// Which kernel: the 256 x 256 tiles where they fill the chip and a row is long enough to repay their 128 KB of LDS (one
+// workgroup a CU); 128 x 128 tiles where those do, at short rows (C's stores bound them, several workgroups a CU overlap);
+// else 16 rows of B at a time, which gives small products workgroups enough.
 template <class T>
 static int launch_matmul(tfrec_ctx *ctx, const MatmulArgs &a)
 {
-    const int64_t tiles = ((a.M + 127) / 128) * ((a.N + 127) / 128);
-    TF_REQUIRE(tiles < (1ll << 31), TFREC_EUNSUP, "the product is too large for one launch");
-    matmul_i8_kernel<T><<<(unsigned)tiles, 256, 0, ctx->stream>>>(a);
+    const int64_t big_m = (a.M + 255) / 256, big_n = (a.N + 255) / 256, mid = ((a.M + 127) / 128) * ((a.N + 127) / 128);
+    if (a.K >= 512 && big_m * big_n >= 160) {
+        TF_REQUIRE(big_m * big_n < (1ll << 28), TFREC_EUNSUP, "the product is too large for one launch");
+        static std::atomic<uint64_t> done{0};
+        TF_TRY(tfrec_raise_lds_limit(ctx, reinterpret_cast<const void *>(&matmul_i8_big_kernel<T>), BIG_LDS, done));
+        const int64_t tiles = big_m * big_n;
+        matmul_i8_big_kernel<T><<<(unsigned)((tiles + 7) / 8 * 8), 512, BIG_LDS, ctx->stream>>>(a, (int)big_m, (int)big_n);
+    } else if (a.M > 128 && mid >= 192) {
+        TF_REQUIRE(mid < (1ll << 31), TFREC_EUNSUP, "the product is too large for one launch");
+        matmul_i8_kernel<T><<<(unsigned)mid, 256, 0, ctx->stream>>>(a);
+    } else {
+        const int64_t nb = (a.N + 15) / 16;
+        TF_REQUIRE(nb < (1ll << 31), TFREC_EUNSUP, "the product is too large for one launch");
+        auto go = [&]<int MT, int KW>() { matmul_i8_rows_kernel<T, MT, KW><<<dim3((unsigned)nb, (unsigned)((a.M + 16 * MT - 1) / (16 * MT))), 64 * KW, 0, ctx->stream>>>(a); };
+        auto waves = [&]<int MT>() {
+            if (a.K <= 256) go.template operator()<MT, 1>();
+            else if (a.K <= 2048 || MT == 8) go.template operator()<MT, 4>();
+            else if constexpr (MT < 8) go.template operator()<MT, 8>();
+        };
+        if (a.M <= 16) waves.template operator()<1>();
+        else if (a.M <= 32) waves.template operator()<2>();
+        else if (a.M <= 64) waves.template operator()<4>();
+        else waves.template operator()<8>();
+    }
     TF_HIP(hipGetLastError());
     return TFREC_OK;
 }

@@ -21,6 +21,8 @@
 typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
 typedef int32_t i32x16 __attribute__((ext_vector_type(16)));
 
+struct __attribute__((packed, aligned(4))) Float4 { float v[4]; };       // 16 bytes at the alignment of a float
+
 static constexpr int BLOCK = 32, CELL = 16;    // items per block (a matrix instruction's rows) and per cell
 static constexpr int SMALL_ITEMS = 4096;       // (16 scores per thread of score_small_i8_kernel)
 static constexpr uint32_t KEY_NONE = 0x007fffffu;      // orderable form of -inf: nothing below or at it is listed
@@ -82,7 +84,8 @@ struct RowDot {
 // ------------------------------------------------------------------------------------------
 struct MaxArgs {
     ScoreI8Args s;
-    float *bound;              // [n, pitch]
+    float *bound;              // [n, pitch]: cells
+    float *group_bound;        // [n, groups]: the largest bound of a group's 16 cells
     float *slack;              // [n, splits]: 1.6 sp sq, the largest over a split
     int64_t pitch;             // cells per user row: 16 per group of 8 blocks
     int64_t groups;            // groups of 8 blocks
@@ -114,6 +117,7 @@ __global__ __launch_bounds__(256, 2) void score_max_i8_kernel(MaxArgs m)
 {
     __shared__ float out[4][UW][16][32];
     __shared__ __align__(16) float scales[4][2][64];
+    __shared__ float tops[4][UW][4][32];
     const ScoreI8Args &a = m.s;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 31, h = lane >> 5;
     // consecutive workgroups go to the 8 XCDs in turn: an XCD takes every 8th slice of the items, for all users one after
@@ -250,6 +254,19 @@ __global__ __launch_bounds__(256, 2) void score_max_i8_kernel(MaxArgs m)
                 float4 *to = reinterpret_cast<float4 *>(m.bound + ur * m.pitch + g * 16 + 8 * h);
                 to[0] = make_float4(v[0], v[1], v[2], v[3]);
                 to[1] = make_float4(v[4], v[5], v[6], v[7]);
+            }
+            float top = fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
+            top = fmaxf(top, __uint_as_float(swap32(__float_as_uint(top), lane)));
+            // four groups' bounds are stored together: one store per row and group would be as many as the cells take
+            const int at = (int)(g - g0) & 3;
+            tops[wave][s][at][r] = top;
+            if (at == 3 || g + 1 == g1) {
+                float *to = m.group_bound + ur * m.groups + g - at;
+                if (h == 0 && ur < a.n) {
+                    if (at == 3) *reinterpret_cast<Float4 *>(to) = Float4{{tops[wave][s][0][r], tops[wave][s][1][r], tops[wave][s][2][r], top}};
+                    else
+                        for (int j = 0; j <= at; ++j) to[j] = tops[wave][s][j][r];
+                }
             }
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -400,8 +417,11 @@ __device__ __forceinline__ void group_finish(GroupList<LIST> &g, const ScoreI8Ar
 // ------------------------------------------------------------------------------------------
 // step 2: the cells that can hold a listed item, scored again
 // ------------------------------------------------------------------------------------------
-static constexpr int SLICES = 1024;            // groups of cells: cell y belongs to slice y % SLICES
-static constexpr int CAND = 1024;              // cells per round
+// The cut is taken over groups of 16 cells where there are groups enough (a sixteenth of the bounds is then read), else over
+// the cells themselves: "units" below.
+static constexpr int SLICES = 1024;            // unit u belongs to slice u % SLICES
+static constexpr int UNITS = 2048;             // units listed at a time
+static constexpr int CAND = 2048;              // cells scored between two looks at the lists
 
 // first item of cell y, and item e of it
 __device__ __forceinline__ int64_t cell_first(int64_t y) { return (y >> 1) * BLOCK + 4 * (y & 1); }
@@ -412,10 +432,10 @@ template <int NT, int LPI, int LIST>
 __global__ __launch_bounds__(NT) void pick_i8_kernel(MaxArgs m)
 {
     __shared__ GroupList<LIST> g;
-    __shared__ uint32_t cand[CAND];
+    __shared__ uint32_t cand[CAND], units[UNITS];
     __shared__ uint16_t slices[SLICES];
     __shared__ uint8_t train[SLICES];
-    __shared__ int n_slices, n_cand;
+    __shared__ int n_slices, n_units, n_cand;
     __shared__ float slack;
     constexpr int V = SLICES / NT;
     const ScoreI8Args &a = m.s;
@@ -427,8 +447,11 @@ __global__ __launch_bounds__(NT) void pick_i8_kernel(MaxArgs m)
     dot.init(a, prow);
     const int64_t mlo = a.train_indptr ? a.train_indptr[user] : 0, mhi = a.train_indptr ? a.train_indptr[user + 1] : 0;
     const int64_t id0 = a.id_offset + a.item_lo;
-    const uint32_t cells = 2u * (uint32_t)((a.n_items + BLOCK - 1) / BLOCK);
+    const bool by_group = m.groups >= 2 * (a.k + (mhi - mlo)) + 64;
+    const uint32_t count = by_group ? (uint32_t)m.groups : 2u * (uint32_t)((a.n_items + BLOCK - 1) / BLOCK);
     const float *__restrict__ bound = m.bound + r * m.pitch;
+    const float *__restrict__ top = by_group ? m.group_bound + r * m.groups : bound;
+    auto first_id = [&](uint32_t u) { return (int32_t)(id0 + (by_group ? (int64_t)u * (8 * BLOCK) : cell_first(u))); };
     int64_t t = mlo + tid;
     const int32_t train0 = t < mhi ? a.train_indices[t] : -1;
 
@@ -436,27 +459,15 @@ __global__ __launch_bounds__(NT) void pick_i8_kernel(MaxArgs m)
     float mx[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) mx[v] = LOWEST;
-    constexpr int DEPTH = 16 / V > 4 ? 8 : 4;          // loads in flight: DEPTH * V
-    uint32_t y0 = 0;
-    for (; y0 + DEPTH * SLICES <= cells; y0 += DEPTH * SLICES) {
-        float w[DEPTH][V];
-#pragma unroll
-        for (int q = 0; q < DEPTH; ++q)
-#pragma unroll
-            for (int v = 0; v < V; ++v) w[q][v] = bound[y0 + q * SLICES + NT * v + tid];
-#pragma unroll
-        for (int q = 0; q < DEPTH; ++q)
-#pragma unroll
-            for (int v = 0; v < V; ++v) mx[v] = fmaxf(mx[v], w[q][v]);
-    }
-    {
+    constexpr int DEPTH = V >= 4 ? 4 : 8;              // loads in flight: DEPTH * V
+    for (uint32_t u0 = 0; u0 < count; u0 += DEPTH * SLICES) {
         float w[DEPTH][V];
 #pragma unroll
         for (int q = 0; q < DEPTH; ++q)
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                const uint32_t y = y0 + q * SLICES + NT * v + tid;
-                w[q][v] = y < cells ? bound[y] : LOWEST;
+                const uint32_t u = u0 + q * SLICES + NT * v + tid;
+                w[q][v] = u < count ? top[u] : LOWEST;
             }
 #pragma unroll
         for (int q = 0; q < DEPTH; ++q)
@@ -464,7 +475,7 @@ __global__ __launch_bounds__(NT) void pick_i8_kernel(MaxArgs m)
             for (int v = 0; v < V; ++v) mx[v] = fmaxf(mx[v], w[q][v]);
     }
     for (int i = tid; i < SLICES; i += NT) train[i] = 0;
-    if (tid == 0) { g.count = 0; n_slices = 0; n_cand = 0; }
+    if (tid == 0) { g.count = 0; n_slices = 0; n_units = 0; n_cand = 0; }
     if (tid < 64) {
         float w = 0.f;
         for (int i = tid; i < m.splits; i += 64) w = fmaxf(w, m.slack[r * m.splits + i]);
@@ -475,7 +486,7 @@ __global__ __launch_bounds__(NT) void pick_i8_kernel(MaxArgs m)
     // (an index of any other sign or size is another shard's item)
     auto mark = [&](int32_t id) {
         const int64_t i = id - id0;
-        if (id >= 0 && i >= 0 && i < a.n_items) train[(2 * (i / BLOCK) + (i >> 2 & 1)) % SLICES] = 1;
+        if (id >= 0 && i >= 0 && i < a.n_items) train[(by_group ? i / (8 * BLOCK) : 2 * (i / BLOCK) + (i >> 2 & 1)) % SLICES] = 1;
     };
     mark(train0);
     for (t += NT; t < mhi; t += NT) mark(a.train_indices[t]);
@@ -497,60 +508,72 @@ __global__ __launch_bounds__(NT) void pick_i8_kernel(MaxArgs m)
     if (tid == 0) g.kth = T > -INFINITY ? ((uint64_t)f32_orderable(T) << 32) - 1 : ((uint64_t)KEY_NONE << 32 | 0xffffffffu);
     __syncthreads();
 
-    const uint32_t per = (cells + SLICES - 1) / SLICES, total = dot.sp == dot.sp ? (uint32_t)n_slices * per : 0u;
     constexpr int ROUNDS = LPI <= 2 ? 4 : (LPI <= 8 ? 2 : 1);          // rounds of 256 items whose rows are requested together
-    for (uint32_t e0 = 0; e0 < total; e0 += CAND) {
-        const uint64_t kth = g.kth;
-        for (uint32_t i = tid; i < CAND; i += NT) {
-            const uint32_t e = e0 + i;
-            if (e < total) {
-                const uint32_t y = slices[e / per] + (e % per) * SLICES;
-                // the cell's bound under its lowest id: if that is not wanted, nothing in the cell is
-                if (y < cells && make_key(bound[y], (int32_t)(id0 + cell_first(y))) > kth) cand[atomicAdd(&n_cand, 1)] = y;
-            }
+    const int sub = by_group ? 16 : 1;                                  // cells of a unit
+    const uint32_t per = (count + SLICES - 1) / SLICES, total = dot.sp == dot.sp ? (uint32_t)n_slices * per : 0u;
+    for (uint32_t e0 = 0; e0 < total;) {
+        // units of the wanted slices whose bound, under its lowest id, is wanted (else nothing in them is)
+        uint64_t kth = g.kth;
+        const uint32_t e1 = total - e0 < UNITS ? total : e0 + UNITS;
+        for (uint32_t e = e0 + tid; e < e1; e += NT) {
+            const uint32_t u = slices[e / per] + (e % per) * SLICES;
+            if (u < count && make_key(top[u], first_id(u)) > kth) units[atomicAdd(&n_units, 1)] = u;
         }
+        e0 = e1;
         __syncthreads();
-        const int c = n_cand;
-        for (int c0 = 0; c0 < c * CELL; c0 += 256 * ROUNDS) {
-            int acc[ROUNDS];
-            if (tid < 256) {
-                uint4 q[ROUNDS][LPI];
-#pragma unroll
-                for (int o = 0; o < ROUNDS; ++o)
-#pragma unroll
-                    for (int j = 0; j < LPI; ++j) {
-                        const int i = c0 + 256 * o + j * (256 / LPI) + tid / LPI;
-                        int64_t it = i < c * CELL ? cell_item(cand[i / CELL], i % CELL) : 0;
-                        it = it < a.n_items ? it : 0;
-                        q[o][j] = dot.load(a, it);
-                    }
-#pragma unroll
-                for (int o = 0; o < ROUNDS; ++o)
-#pragma unroll
-                    for (int j = 0; j < LPI; ++j) {
-                        const int s = dot.dot(q[o][j]);
-                        if (tid % LPI == j) acc[o] = s;
-                    }
+        const int nu = n_units;
+        for (int v0 = 0; v0 < nu; v0 += CAND / 16) {
+            const int nv = nu - v0 < CAND / 16 ? nu - v0 : CAND / 16;
+            kth = g.kth;
+            for (int i = tid; i < nv * sub; i += NT) {
+                const uint32_t u = units[v0 + i / sub], y = u * sub + i % sub;
+                if (make_key(bound[y], (int32_t)(id0 + cell_first(y))) > kth) cand[atomicAdd(&n_cand, 1)] = y;
             }
-#pragma unroll
-            for (int o = 0; o < ROUNDS; ++o) {
-                if (o > 0 && c0 + 256 * o >= c * CELL) break;
+            __syncthreads();
+            const int c = n_cand;
+            for (int c0 = 0; c0 < c * CELL; c0 += 256 * ROUNDS) {
+                int acc[ROUNDS];
                 if (tid < 256) {
-                    const int i = c0 + 256 * o + RowDot<LPI>::owned();
-                    const int64_t it = i < c * CELL ? cell_item(cand[i / CELL], i % CELL) : a.n_items;
-                    bool pass = false;
-                    uint64_t k64 = 0;
-                    if (it < a.n_items) {
-                        const float v = dot.score(a, acc[o], it);
-                        k64 = make_key(v, (int32_t)(id0 + it));
-                        pass = v > -INFINITY && k64 > g.kth;
-                    }
-                    group_append(g, pass, k64);
+                    uint4 q[ROUNDS][LPI];
+#pragma unroll
+                    for (int o = 0; o < ROUNDS; ++o)
+#pragma unroll
+                        for (int j = 0; j < LPI; ++j) {
+                            const int i = c0 + 256 * o + j * (256 / LPI) + tid / LPI;
+                            int64_t it = i < c * CELL ? cell_item(cand[i / CELL], i % CELL) : 0;
+                            it = it < a.n_items ? it : 0;
+                            q[o][j] = dot.load(a, it);
+                        }
+#pragma unroll
+                    for (int o = 0; o < ROUNDS; ++o)
+#pragma unroll
+                        for (int j = 0; j < LPI; ++j) {
+                            const int s = dot.dot(q[o][j]);
+                            if (tid % LPI == j) acc[o] = s;
+                        }
                 }
-                group_check(g, a.k, a.train_indices, mlo, mhi);
+#pragma unroll
+                for (int o = 0; o < ROUNDS; ++o) {
+                    if (o > 0 && c0 + 256 * o >= c * CELL) break;
+                    if (tid < 256) {
+                        const int i = c0 + 256 * o + RowDot<LPI>::owned();
+                        const int64_t it = i < c * CELL ? cell_item(cand[i / CELL], i % CELL) : a.n_items;
+                        bool pass = false;
+                        uint64_t k64 = 0;
+                        if (it < a.n_items) {
+                            const float v = dot.score(a, acc[o], it);
+                            k64 = make_key(v, (int32_t)(id0 + it));
+                            pass = v > -INFINITY && k64 > g.kth;
+                        }
+                        group_append(g, pass, k64);
+                    }
+                    group_check(g, a.k, a.train_indices, mlo, mhi);
+                }
             }
+            if (tid == 0) n_cand = 0;
+            __syncthreads();
         }
-        if (tid == 0) n_cand = 0;
+        if (tid == 0) n_units = 0;
         __syncthreads();
     }
     group_finish(g, a, r, a.train_indices, mlo, mhi);
@@ -630,7 +653,7 @@ __global__ __launch_bounds__(256) void no_entries_kernel(int32_t *__restrict__ i
 // users per pass of steps 1 and 2: their table of bounds stays below 512 MB (or holds 32 users)
 static int64_t users_per_pass(int64_t n, int64_t groups)
 {
-    int64_t u = ((int64_t)512 << 20) / (groups * 64) / 128 * 128;
+    int64_t u = ((int64_t)512 << 20) / (groups * 68) / 128 * 128;
     u = u < 32 ? 32 : u;
     return n < u ? n : u;
 }
@@ -659,7 +682,7 @@ size_t tfrec_score_i8_bytes(int64_t n, int64_t n_items, int d, int k)
 {
     if (n <= 0 || n_items <= SMALL_ITEMS) return 0;
     const int64_t groups = (n_items + 8 * BLOCK - 1) / (8 * BLOCK), per_pass = users_per_pass(n, groups);
-    return tf_align((size_t)per_pass * groups * 64) + slack_bytes(per_pass, groups, d) + 512;
+    return tf_align((size_t)per_pass * groups * 64) + tf_align((size_t)per_pass * groups * 4) + slack_bytes(per_pass, groups, d) + 1024;
 }
 
 // calls f.operator()<LPI>() with the lanes an item's row takes
@@ -734,9 +757,10 @@ int tfrec_score_i8(tfrec_ctx *ctx, ScoreI8Args a)
     TF_TRY(tfrec_ws_require(ctx, ctx->ws_used + tfrec_score_i8_bytes(a.n, a.n_items, a.d, a.k)));
     TF_TRY(tfrec_note_capture(ctx));
     m.bound = (float *)tfrec_ws_take(ctx, (size_t)per_pass * m.pitch * 4);
+    m.group_bound = (float *)tfrec_ws_take(ctx, (size_t)per_pass * m.groups * 4);
     const size_t slack = slack_bytes(per_pass, m.groups, a.d);
     m.slack = (float *)tfrec_ws_take(ctx, slack);
-    TF_REQUIRE(m.bound != nullptr && m.slack != nullptr, TFREC_ENOMEM, "internal: workspace carve failed");
+    TF_REQUIRE(m.bound != nullptr && m.group_bound != nullptr && m.slack != nullptr, TFREC_ENOMEM, "internal: workspace carve failed");
     for (int64_t u0 = 0; u0 < a.n; u0 += per_pass) {
         m.s = a;
         m.s.n = a.n - u0 < per_pass ? a.n - u0 : per_pass;

@@ -2,6 +2,8 @@
 #pragma once
 #include "common.hpp"
 
+#include <atomic>
+
 struct ScoreI8Args {
     const int8_t *Pq;          // user rows: the table [U, ldp], or the listed users' rows in order (p_compact)
     int64_t ldp;
@@ -24,6 +26,8 @@ struct ScoreI8Args {
     uint32_t *flags;
 };
 
+// raises a kernel's dynamic-LDS limit once per device (eval.hip)
+int tfrec_raise_lds_limit(tfrec_ctx *ctx, const void *kernel, int bytes, std::atomic<uint64_t> &done);
 // the layout every 8-bit matrix has to have (quant.hip)
 int tfrec_check_i8(const char *name, const int8_t *q, int64_t rows, int64_t ld, int64_t cols);
 // tfrec_quantize_rows_i8 without the checks (quant.hip)
