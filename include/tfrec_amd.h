@@ -341,10 +341,22 @@ int tfrec_grad_norm(tfrec_ctx *ctx, int n, const void *const *h_grads, const int
  * left as it is.  A norm that is infinite or not a number makes every value NaN.  h_out[i] may be
  * h_grads[i]; apart from that no output may overlap another output or any gradient (TFREC_EINVAL).  d_norm (the norm
  * before scaling) may be null.  max_norm: positive and finite.
- * Both calls use fixed scratch of the context, never its workspace, and can be captured into a HIP graph; graphs
+ * These calls use fixed scratch of the context, never its workspace, and can be captured into a HIP graph; graphs
  * captured from one context share that scratch and must not be replayed at the same time. */
 int tfrec_grad_clip(tfrec_ctx *ctx, int n, const void *const *h_grads, void *const *h_out, const int64_t *h_counts,
                     const int *h_dtypes, float max_norm, float *d_norm);
+
+/* The same on a list that is kept: a program that steps on the same gradient buffers makes one list, and a step is then
+ * one launch for a few ten thousand values and two for any other number, whatever the number of tensors.
+ *   tfrec_grads_create   checks the arguments as tfrec_grad_clip does and lays the list out on the device (synchronous;
+ *                        not under stream capture); the buffers have to outlive it, the host arrays need not
+ *   tfrec_grads_destroy  waits for the context's stream (a null context: for the device) and frees it */
+typedef struct tfrec_grads tfrec_grads;
+int tfrec_grads_create(tfrec_ctx *ctx, int n, const void *const *h_grads, void *const *h_out, const int64_t *h_counts,
+                       const int *h_dtypes, tfrec_grads **out);
+int tfrec_grads_destroy(tfrec_ctx *ctx, tfrec_grads *g);
+int tfrec_grads_norm(tfrec_ctx *ctx, const tfrec_grads *g, float *d_norm);
+int tfrec_grads_clip(tfrec_ctx *ctx, const tfrec_grads *g, float max_norm, float *d_norm);
 
 /* ---- 8-bit rows ------------------------------------------------------------------------------- */
 /* A matrix in 8-bit integers with one float32 scale per row: value = q * scale.  Rows are ldq bytes apart, ldq a

@@ -52,10 +52,18 @@ def run_clip(dev, host, max_norm, in_place):
         close(g, x, s, exact=want_norm <= max_norm)
     if not in_place:
         assert all(torch.equal(g.cpu(), x) for g, x in zip(grads, host))
+    # a kept list gives the same
+    again = [x.cuda() for x in host]
+    lst = dev.grad_list(again, out=None if in_place else [torch.full_like(x, 5.0) for x in again])
+    n2 = dev.grad_norm(lst, norm=torch.zeros(1).cuda())
+    n3 = dev.clip_grads(lst, max_norm, norm=torch.zeros(1).cuda())
+    assert abs(float(n2) - want_norm) <= 2.0 ** -23 * want_norm and abs(float(n3) - want_norm) <= 2.0 ** -23 * want_norm
+    for g, x in zip(lst.out, host):
+        close(g, x, s, exact=want_norm <= max_norm)
     assert float(dev.grad_norm(grads if not in_place else [x.cuda() for x in host], norm=torch.zeros(1).cuda())) == float(norm)
 
 
-LENGTHS = [[1], [0], [0, 3, 0], [17], [255, 1, 4096], [8191], [8192], [8193, 8192, 1], [100003], [7] * 95, [11] * 96, [5] * 97, [3, 20000] * 150, [3_000_001, 2, 50]]
+LENGTHS = [[1], [0], [60000, 5000], [8192 * 8], [8192 * 8 + 1], [9000, 9000, 9000, 1], [0, 3, 0], [17], [255, 1, 4096], [8191], [8192], [8193, 8192, 1], [100003], [7] * 95, [11] * 96, [5] * 97, [3, 20000] * 150, [3_000_001, 2, 50]]
 
 
 @pytest.mark.parametrize("in_place", [True, False])
@@ -205,7 +213,7 @@ def test_bpr_grads(dev, U, I, d, B):
         tol = 2.0 ** -23 * (12 * np.sqrt(most) + 8) * max(1.0, float(w.abs().max()))
         assert float((g.cpu().double() - w).abs().max()) <= tol, (float((g.cpu().double() - w).abs().max()), tol)
     if B:
-        assert abs(float(loss[0]) - float(total - reg * l2)) <= 1e-5 * abs(float(total)) and abs(float(loss[1]) - float(l2)) <= 1e-5 * float(l2)
+        assert abs(float(loss[0]) - float((total - reg * l2).detach())) <= 1e-5 * abs(float(total.detach())) and abs(float(loss[1]) - float(l2.detach())) <= 1e-5 * float(l2.detach())
     # the step is the parameters plus -lr times these gradients, bit for bit
     a, c = [t.clone() for t in gpu[:3]], [t.clone() for t in gpu[:3]]
     dev.bpr_sgd_step(*a, *gpu[3:], 0.02, reg)
@@ -237,3 +245,97 @@ def test_bpr_grads_refusals(dev):
         dev.bpr_grads(P, Q, b, e, e, e, 0.0, P, torch.zeros_like(Q), torch.zeros_like(b))
     with pytest.raises(ValueError, match="shapes"):
         dev.bpr_grads(P, Q, b, e, e, e, 0.0, torch.zeros(3, 8).cuda(), torch.zeros_like(Q), torch.zeros_like(b))
+
+
+# ------------------------------------------------------------------------------------------------------------- models
+class _Data:
+    def __init__(self, train, test):
+        self.train_matrix, self.test_matrix = train, test
+
+
+class _Log:
+    def __init__(self):
+        self.lines = []
+
+    def info(self, s):
+        self.lines.append(s)
+
+
+def small_data():
+    import scipy.sparse as sp
+    rng = np.random.default_rng(5)
+    dense = rng.random((60, 90))
+    return _Data(sp.csr_matrix((dense < 0.1).astype(np.float32)), sp.csr_matrix(((dense > 0.1) & (dense < 0.15)).astype(np.float32)))
+
+
+def make_model(name, data, evaluator, **more):
+    from tfrec_amd.device import Device
+    from tfrec_amd.model.BPR import BPR
+    from tfrec_amd.model.DNSBPR import DNSBPR
+    cls = {"BPR": BPR, "DNSBPR": DNSBPR}[name]
+    cls.logger = _Log()
+    config = dict(factors_num=12, lr=0.05, reg=0.01, epochs=2, batch_size=64, neg_num=4, data_name="t", **more)
+    return cls(Device(0), config, data, evaluator)
+
+
+@pytest.mark.parametrize("name", ["BPR", "DNSBPR"])
+@pytest.mark.parametrize("sampler", ["host", "device"])
+def test_a_bound_that_no_batch_reaches_changes_nothing(name, sampler, tmp_path, monkeypatch):
+    from tfrec_amd.evaluator import FoldOutEvaluator
+    monkeypatch.chdir(tmp_path)                 # (DNSBPR leaves its parameters in a file)
+    data, tables = small_data(), []
+    for bound in (0, 1e6):
+        np.random.seed(11)
+        m = make_model(name, data, FoldOutEvaluator(data.train_matrix, data.test_matrix, top_k=10), sampler=sampler, clip_norm=bound)
+        m.train_model()
+        tables.append(m.parameters())
+    assert all(np.array_equal(a, b) for a, b in zip(*tables))
+
+
+def test_clipped_steps_and_8_bit_evaluation_run_together(tmp_path, monkeypatch):
+    """A model trained under a bound that every batch reaches, evaluated with 8-bit scores: the tables against the same steps
+    in float64, the lists behind the metrics against the definition of the scores."""
+    from tfrec_amd.evaluator import FoldOutEvaluator
+    data = small_data()
+    bound = 0.25
+    ev = FoldOutEvaluator.from_config({"score_dtype": "i8", "top_k": 10}, data.train_matrix, data.test_matrix)
+    m = make_model("BPR", data, ev, clip_norm=bound, sampler="device")
+    P, Q, b = [torch.from_numpy(x).double() for x in m.parameters()]
+    users, pos, neg = [torch.from_numpy(x.numpy()).long().reshape(-1) for x in m._device_epoch(0)]
+    m._train_epoch_on_device(0)
+    n, clipped = m._device_sampler.nnz, 0
+    for lo in range(0, n, 64):
+        leaves = [t.clone().requires_grad_() for t in (P, Q, b)]
+        s = slice(lo, min(lo + 64, n))
+        grads = torch.autograd.grad(bpr_loss(*leaves, users[s], pos[s], neg[s], 0.01)[0], leaves)
+        norm = float(torch.sqrt(sum((g * g).sum() for g in grads)))
+        clipped += norm > bound
+        P, Q, b = [t - 0.05 * g * (bound / max(norm, bound)) for t, g in zip((P, Q, b), grads)]
+    assert clipped == (n + 63) // 64
+    got = m.parameters()
+    # every step moves a value by at most 0.05 * 0.25, in float32 arithmetic of a few roundings; so do the steps before it
+    for g, w in zip(got, (P, Q, b)):
+        assert float(np.abs(g - w.numpy()).max()) <= (n // 64 + 1) * 0.05 * bound * 2.0 ** -20
+    curves = ev.evaluate(m).reshape(5, 10)
+    scores = m.mf.all_logits(score_dtype="i8")
+    hits = []
+    for u in range(60):
+        test = data.test_matrix[u].indices
+        if len(test):
+            row = scores[u].copy()
+            row[data.train_matrix[u].indices] = -np.inf
+            top = np.lexsort((np.arange(90), -row))[:10]
+            hits.append([np.isin(top[:j + 1], test).mean() for j in range(10)])
+    np.testing.assert_allclose(curves[0], np.mean(hits, 0), rtol=1e-5)
+    near = np.abs(m.mf.all_logits() - scores).max()
+    # half a step of either row on every product: |p| |q| d / 254 each way
+    assert near <= 12 * 2 * np.abs(got[0]).max() * np.abs(got[1]).max() / 254 * 1.01 + 1e-6
+    assert np.array_equal(m.mf.all_logits([5, 3, 5], score_dtype="i8"), scores[[5, 3, 5]])
+
+
+def test_clip_norm_of_sharded_and_adversarial_models_is_refused():
+    from tfrec_amd.evaluator import FoldOutEvaluator
+    data = small_data()
+    ev = FoldOutEvaluator(data.train_matrix, data.test_matrix, top_k=5)
+    with pytest.raises(ValueError, match="single-GPU"):
+        make_model("BPR", data, ev, clip_norm=1.0, force_sharded=True)

@@ -210,3 +210,32 @@ def test_python_refusals():
         GradList(Dev(), [torch.zeros(3, dtype=torch.float64)])
     with pytest.raises(ValueError, match="1 outputs for 2"):
         GradList(Dev(), [torch.zeros(3), torch.zeros(3)], out=[torch.zeros(3)])
+
+
+def test_configuration_refusals():
+    from tfrec_amd.model.APR import APR
+    from tfrec_amd.model.BPR import clip_norm_of
+    assert clip_norm_of({}) == 0.0 and clip_norm_of({"clip_norm": 2}) == 2.0
+    for bad in (-1.0, float("nan"), float("inf"), "1.0", None, True):
+        with pytest.raises(ValueError, match="clip_norm"):
+            clip_norm_of({"clip_norm": bad})
+    with pytest.raises(ValueError, match="BPR and DNSBPR"):
+        APR(None, {"clip_norm": 1.0}, None, None)
+    import scipy.sparse as sp
+    from tfrec_amd.evaluator import FoldOutEvaluator
+    m = sp.csr_matrix(np.eye(3, dtype=np.float32))
+    assert FoldOutEvaluator.from_config({"score_dtype": "i8"}, m, m).score_mode == _lib.SCORE_I8
+    with pytest.raises(ValueError, match="score_dtype"):
+        FoldOutEvaluator(m, m, score_dtype="i4")
+
+
+def test_list_refusals(lib):
+    h = C.c_void_p()
+    one = (C.c_void_p * 1)(A16), (C.c_void_p * 1)(A16 + 4), (C.c_int64 * 1)(4), (C.c_int * 1)(0)
+    refused(lib, lib.tfrec_grads_create(None, 1, *one, C.byref(h)), _lib.EINVAL, "does not replace")
+    refused(lib, lib.tfrec_grads_create(None, 1, one[0], one[0], one[2], one[3], None), _lib.EINVAL, "out is null")
+    refused(lib, lib.tfrec_grads_create(None, 1, one[0], one[0], one[2], one[3], C.byref(h)), _lib.EINVAL, "null context")
+    assert h.value is None
+    refused(lib, lib.tfrec_grads_norm(None, None, A16), _lib.EINVAL, "null list")
+    refused(lib, lib.tfrec_grads_clip(None, None, 1.0, A16), _lib.EINVAL, "null list")
+    assert lib.tfrec_grads_destroy(None, None) == _lib.OK

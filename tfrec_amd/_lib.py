@@ -73,6 +73,10 @@ SIGNATURES = {
     "tfrec_bpr_grads": (_int, [_p, _p, _p, _p, _i64, _i64, _int, _p, _p, _p, _i64, _f, _p, _p, _p, _p]),
     "tfrec_grad_norm": (_int, [_p, _int, _p, _p, _p, _p]),
     "tfrec_grad_clip": (_int, [_p, _int, _p, _p, _p, _p, _f, _p]),
+    "tfrec_grads_create": (_int, [_p, _int, _p, _p, _p, _p, C.POINTER(_p)]),
+    "tfrec_grads_destroy": (_int, [_p, _p]),
+    "tfrec_grads_norm": (_int, [_p, _p, _p]),
+    "tfrec_grads_clip": (_int, [_p, _p, _f, _p]),
     "tfrec_quantize_rows_i8": (_int, [_p, _p, _int, _i64, _i64, _i64, _p, _i64, _p, _i64, _p]),
     "tfrec_matmul_i8": (_int, [_p, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _i64, _p, _p, _int, _i64]),
     "tfrec_score_topk_i8": (_int, [_p, _p, _i64, _p, _i64, _int, _p, _i64, _p, _p, _i64, _int, _i64, _i64, _p, _i64, _p, _p, _int, _p, _p]),

@@ -8,11 +8,28 @@
 // float32 value's square leaves its range, and the sum of 10^9 values keeps more bits than the result has.
 #include "common.hpp"
 
-static constexpr int GRAD_TENSORS = 96;        // tensors per launch: their table rides in the kernel's arguments (below 4 KB)
+static constexpr int GRAD_TENSORS = 96;        // tensors per launch of a call without a list: their table rides in the kernel's arguments (below 4 KB)
 static constexpr int GRAD_CHUNK = 8192;        // values per chunk
-static constexpr int GRAD_BLOCKS = 1024;       // partial sums (and workgroups at most)
+static constexpr int GRAD_BLOCKS = 2048;       // partial sums (and workgroups at most)
+static constexpr int GRAD_SMALL = 8;           // chunks one workgroup holds in its registers
 static_assert(GRAD_BLOCKS * sizeof(double) <= TFREC_SMALL_BYTES, "partial sums exceed the context's scratch");
 
+// a chunk: `len` values of one tensor
+struct GradChunk {
+    const void *src;
+    void *dst;
+    int32_t len, dtype;
+    int64_t unused;                            // (32 bytes: one scalar load)
+};
+
+// where a kernel finds chunk c: in a list on the device ...
+struct GradListed {
+    const GradChunk *at;
+    int64_t chunks;
+    __device__ __forceinline__ GradChunk get(int64_t c) const { return at[c]; }
+};
+
+// ... or by a search among the tensors of a table in its arguments
 struct GradTable {
     const void *src[GRAD_TENSORS];
     void *dst[GRAD_TENSORS];
@@ -21,21 +38,30 @@ struct GradTable {
     uint8_t dtype[GRAD_TENSORS];
     int n;
     int64_t chunks;
+    __device__ __forceinline__ GradChunk get(int64_t c) const
+    {
+        int lo = 0, hi = n;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (first[mid] <= c) lo = mid; else hi = mid;
+        }
+        const int64_t at = (c - first[lo]) * GRAD_CHUNK, left = count[lo] - at, es = dtype[lo] == TFREC_DT_F32 ? 4 : 2;
+        return GradChunk{(const char *)src[lo] + at * es, dst[lo] ? (char *)dst[lo] + at * es : nullptr, (int32_t)(left < GRAD_CHUNK ? left : GRAD_CHUNK),
+                         dtype[lo], 0};
+    }
 };
 
 // 16 bytes at the alignment of the element type (global memory takes them at any)
 template <class T>
 struct __attribute__((packed, aligned(sizeof(T)))) Pack { T v[16 / sizeof(T)]; };
 
-// tensor of chunk c (wave-uniform)
-__device__ __forceinline__ int tensor_of(const GradTable &t, int64_t c)
+// f.operator()<T>(src, dst) with the chunk's type
+template <class F>
+__device__ __forceinline__ void by_type(const GradChunk &c, F &&f)
 {
-    int lo = 0, hi = t.n;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (t.first[mid] <= c) lo = mid; else hi = mid;
-    }
-    return lo;
+    if (c.dtype == TFREC_DT_F32) f.template operator()<float>((const float *)c.src, (float *)c.dst);
+    else if (c.dtype == TFREC_DT_BF16) f.template operator()<__bf16>((const __bf16 *)c.src, (__bf16 *)c.dst);
+    else f.template operator()<_Float16>((const _Float16 *)c.src, (_Float16 *)c.dst);
 }
 
 template <class T>
@@ -75,31 +101,47 @@ __device__ __forceinline__ void chunk_scale(const T *x, T *y, int m, float s, fl
     }
 }
 
-// sum over the 256 threads, the same on every thread, in a fixed order
+// sum over the workgroup's NW waves, the same on every thread, in a fixed order
+template <int NW>
 __device__ __forceinline__ double block_sum(double v)
 {
-    __shared__ double red[4];
+    __shared__ double red[NW];
     for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
-    v = (red[0] + red[1]) + (red[2] + red[3]);
+    v = 0.;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) v += red[w];
     __syncthreads();
     return v;
 }
 
+// The factor of every value, as s * p2.  (A sum of squares of finite float32 values stays finite in float64: a norm that is
+// not finite means an infinity or NaN among the values.)  A factor near or below the subnormal range of float32 (gradients
+// of 1e35 and more) is applied as s 2^64 and then 2^-64.
+struct GradFactor {
+    float s, p2;
+    __device__ __forceinline__ GradFactor(double norm, double max_norm)
+    {
+        const double f = norm <= max_norm ? 1. : max_norm / norm;
+        const bool tiny = f < 0x1p-100;
+        s = !(norm < (double)INFINITY) ? NAN : (float)(tiny ? f * 0x1p64 : f);
+        p2 = tiny ? 0x1p-64f : 1.f;
+    }
+    // in place and within the bound: every value is what it was
+    __device__ __forceinline__ bool nothing(const GradChunk &c) const { return s == 1.f && c.src == c.dst; }
+};
+
 // partial sum of workgroup b over its chunks b, b + grid, ...; `first`: the first launch of a call, which sets the partials
-__global__ __launch_bounds__(256) void grad_squares_kernel(GradTable t, double *__restrict__ part, int first)
+template <class Table>
+__global__ __launch_bounds__(256) void grad_squares_kernel(Table t, double *__restrict__ part, int first)
 {
     double s = 0.;
-    for (int64_t c = blockIdx.x; c < t.chunks; c += gridDim.x) {
-        const int i = tensor_of(t, c);
-        const int64_t at = (c - t.first[i]) * GRAD_CHUNK, left = t.count[i] - at;
-        const int m = left < GRAD_CHUNK ? (int)left : GRAD_CHUNK;
-        if (t.dtype[i] == TFREC_DT_F32) s = chunk_squares((const float *)t.src[i] + at, m, s);
-        else if (t.dtype[i] == TFREC_DT_BF16) s = chunk_squares((const __bf16 *)t.src[i] + at, m, s);
-        else s = chunk_squares((const _Float16 *)t.src[i] + at, m, s);
+    for (int64_t k = blockIdx.x; k < t.chunks; k += gridDim.x) {
+        const GradChunk c = t.get(k);
+        by_type(c, [&]<class T>(const T *x, T *) { s = chunk_squares(x, c.len, s); });
     }
-    s = block_sum(s);
+    s = block_sum<4>(s);
     if (threadIdx.x == 0) part[blockIdx.x] = first ? s : part[blockIdx.x] + s;
 }
 
@@ -108,7 +150,7 @@ __device__ __forceinline__ double norm_of(const double *__restrict__ part, int n
 {
     double s = 0.;
     for (int i = threadIdx.x; i < n_part; i += 256) s += part[i];
-    return sqrt(block_sum(s));
+    return sqrt(block_sum<4>(s));
 }
 
 __global__ __launch_bounds__(256) void grad_norm_kernel(const double *__restrict__ part, int n_part, float *__restrict__ norm)
@@ -117,25 +159,80 @@ __global__ __launch_bounds__(256) void grad_norm_kernel(const double *__restrict
     if (threadIdx.x == 0) *norm = (float)nm;
 }
 
-__global__ __launch_bounds__(256) void grad_scale_kernel(GradTable t, const double *__restrict__ part, int n_part, double max_norm, float *__restrict__ norm)
+template <class Table>
+__global__ __launch_bounds__(256) void grad_scale_kernel(Table t, const double *__restrict__ part, int n_part, double max_norm, float *__restrict__ norm)
 {
     const double nm = norm_of(part, n_part);
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)nm;
-    // (a sum of squares of finite float32 values stays finite in float64: not finite = an infinity or NaN among the values)
-    // A scale near or below the subnormal range of float32 (gradients of 1e35 and more) is applied as s 2^64 and then 2^-64.
-    const double sd = nm <= max_norm ? 1. : max_norm / nm;
-    const bool tiny = sd < 0x1p-100;
-    const float s = !(nm < (double)INFINITY) ? NAN : (float)(tiny ? sd * 0x1p64 : sd), p2 = tiny ? 0x1p-64f : 1.f;
+    const GradFactor f(nm, max_norm);
     // the last chunks first: what the norm read last is still cached
     for (int64_t k = blockIdx.x; k < t.chunks; k += gridDim.x) {
-        const int64_t c = t.chunks - 1 - k;
-        const int i = tensor_of(t, c);
-        if (s == 1.f && t.src[i] == t.dst[i]) continue;        // in place and within the bound: every value is what it was
-        const int64_t at = (c - t.first[i]) * GRAD_CHUNK, left = t.count[i] - at;
-        const int m = left < GRAD_CHUNK ? (int)left : GRAD_CHUNK;
-        if (t.dtype[i] == TFREC_DT_F32) chunk_scale((const float *)t.src[i] + at, (float *)t.dst[i] + at, m, s, p2);
-        else if (t.dtype[i] == TFREC_DT_BF16) chunk_scale((const __bf16 *)t.src[i] + at, (__bf16 *)t.dst[i] + at, m, s, p2);
-        else chunk_scale((const _Float16 *)t.src[i] + at, (_Float16 *)t.dst[i] + at, m, s, p2);
+        const GradChunk c = t.get(t.chunks - 1 - k);
+        if (!f.nothing(c)) by_type(c, [&]<class T>(const T *x, T *y) { chunk_scale(x, y, c.len, f.s, f.p2); });
+    }
+}
+
+// Few values: one workgroup holds all of them in registers between the norm and the product (one launch, one read).
+template <class Table>
+__global__ __launch_bounds__(1024) void grad_clip_small_kernel(Table t, double max_norm, float *__restrict__ norm)
+{
+    uint4 held[GRAD_SMALL][2];                 // 8 values of each chunk: two packs of 4, or one of 8
+    double s = 0.;
+    const int n = (int)t.chunks;
+#pragma unroll
+    for (int k = 0; k < GRAD_SMALL; ++k) {
+        if (k >= n) break;
+        const GradChunk c = t.get(k);
+        by_type(c, [&]<class T>(const T *x, T *) {
+            constexpr int V = 16 / sizeof(T), R = 8 / V;
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const int i = (r * 1024 + threadIdx.x) * V;
+                Pack<T> p;
+                if (i + V <= c.len) p = *reinterpret_cast<const Pack<T> *>(x + i);
+                else
+#pragma unroll
+                    for (int j = 0; j < V; ++j) p.v[j] = i + j < c.len ? x[i + j] : (T)0.f;
+                held[k][r] = __builtin_bit_cast(uint4, p);
+            }
+        });
+    }
+#pragma unroll
+    for (int k = 0; k < GRAD_SMALL; ++k) {
+        if (k >= n) break;
+        const GradChunk c = t.get(k);
+        by_type(c, [&]<class T>(const T *, T *) {
+            constexpr int V = 16 / sizeof(T), R = 8 / V;
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const Pack<T> p = __builtin_bit_cast(Pack<T>, held[k][r]);
+#pragma unroll
+                for (int j = 0; j < V; ++j) { const double v = (double)(float)p.v[j]; s = fma(v, v, s); }
+            }
+        });
+    }
+    const double nm = sqrt(block_sum<16>(s));
+    if (norm && threadIdx.x == 0) *norm = (float)nm;
+    const GradFactor f(nm, max_norm);
+#pragma unroll
+    for (int k = 0; k < GRAD_SMALL; ++k) {
+        if (k >= n) break;
+        const GradChunk c = t.get(k);
+        if (f.nothing(c)) continue;
+        by_type(c, [&]<class T>(const T *, T *y) {
+            constexpr int V = 16 / sizeof(T), R = 8 / V;
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const int i = (r * 1024 + threadIdx.x) * V;
+                Pack<T> p = __builtin_bit_cast(Pack<T>, held[k][r]);
+#pragma unroll
+                for (int j = 0; j < V; ++j) p.v[j] = (T)((float)p.v[j] * f.s * f.p2);
+                if (i + V <= c.len) *reinterpret_cast<Pack<T> *>(y + i) = p;
+                else
+                    for (int j = 0; j < V; ++j)
+                        if (i + j < c.len) y[i + j] = p.v[j];
+            }
+        });
     }
 }
 
@@ -231,57 +328,43 @@ static int for_tables(int n, const void *const *g, void *const *out, const int64
     return flush();
 }
 
-// leaves the partial sums in the context's scratch; *n_part = how many
-static int grad_squares(tfrec_ctx *ctx, int n, const void *const *g, const int64_t *counts, const int *dtypes, int *n_part)
+// One launch sequence over `tables` tables (each(f) calls f(table) for every one of them): the partial sums, then what the
+// call wants of them.  `most`: the largest number of chunks of a table; `total`: of all.
+template <class Each>
+static int run_norm(tfrec_ctx *ctx, int64_t most, Each &&each, int *n_part)
 {
-    int64_t most = 1;
-    TF_TRY(for_tables(n, g, nullptr, counts, dtypes, [&](const GradTable &t) -> int { most = t.chunks > most ? t.chunks : most; return TFREC_OK; }));
-    const int blocks = most < GRAD_BLOCKS ? (int)most : GRAD_BLOCKS;
+    const int blocks = most < 1 ? 1 : (most < GRAD_BLOCKS ? (int)most : GRAD_BLOCKS);
     double *part = (double *)ctx->d_small;
     int first = 1;
-    TF_TRY(for_tables(n, g, nullptr, counts, dtypes, [&](const GradTable &t) -> int {
+    TF_TRY(each([&](const auto &t) -> int {
         grad_squares_kernel<<<blocks, 256, 0, ctx->stream>>>(t, part, first);
         TF_HIP(hipGetLastError());
         first = 0;
         return TFREC_OK;
     }));
     if (first) {                                   // nothing but empty tensors
-        GradTable t;
-        t.n = 0;
-        t.chunks = 0;
-        grad_squares_kernel<<<blocks, 256, 0, ctx->stream>>>(t, part, 1);
+        grad_squares_kernel<<<blocks, 256, 0, ctx->stream>>>(GradListed{nullptr, 0}, part, 1);
         TF_HIP(hipGetLastError());
     }
     *n_part = blocks;
     return TFREC_OK;
 }
 
-extern "C" int tfrec_grad_norm(tfrec_ctx *ctx, int n, const void *const *h_grads, const int64_t *h_counts, const int *h_dtypes, float *d_norm)
+template <class Each>
+static int run_clip(tfrec_ctx *ctx, int64_t most, int tables, Each &&each, float max_norm, float *d_norm)
 {
-    TF_TRY(check_grads(n, h_grads, h_counts, h_dtypes));
-    TF_REQUIRE(d_norm && ((uintptr_t)d_norm & 3u) == 0, TFREC_EINVAL, "null or misaligned output");
-    TF_TRY(tfrec_ctx_enter(ctx));
+    if (tables == 1 && most <= GRAD_SMALL)
+        return each([&](const auto &t) -> int {
+            grad_clip_small_kernel<<<1, 1024, 0, ctx->stream>>>(t, (double)max_norm, d_norm);
+            TF_HIP(hipGetLastError());
+            return TFREC_OK;
+        });
     int n_part = 0;
-    TF_TRY(grad_squares(ctx, n, h_grads, h_counts, h_dtypes, &n_part));
-    grad_norm_kernel<<<1, 256, 0, ctx->stream>>>((const double *)ctx->d_small, n_part, d_norm);
-    TF_HIP(hipGetLastError());
-    return TFREC_OK;
-}
-
-extern "C" int tfrec_grad_clip(tfrec_ctx *ctx, int n, const void *const *h_grads, void *const *h_out, const int64_t *h_counts,
-                               const int *h_dtypes, float max_norm, float *d_norm)
-{
-    TF_TRY(check_grads(n, h_grads, h_counts, h_dtypes));
-    TF_REQUIRE(max_norm > 0.f && max_norm < INFINITY, TFREC_EINVAL, "max_norm must be positive and finite, got %g", (double)max_norm);
-    TF_REQUIRE(((uintptr_t)d_norm & 3u) == 0, TFREC_EINVAL, "misaligned output");
-    TF_TRY(check_outputs(n, h_grads, h_out, h_counts, h_dtypes));
-    TF_TRY(tfrec_ctx_enter(ctx));
-    int n_part = 0;
-    TF_TRY(grad_squares(ctx, n, h_grads, h_counts, h_dtypes, &n_part));
+    TF_TRY(run_norm(ctx, most, each, &n_part));
     const double *part = (const double *)ctx->d_small;
     bool any = false;
-    TF_TRY(for_tables(n, h_grads, h_out, h_counts, h_dtypes, [&](const GradTable &t) -> int {
-        const int blocks = t.chunks < 2 * GRAD_BLOCKS ? (int)t.chunks : 2 * GRAD_BLOCKS;
+    TF_TRY(each([&](const auto &t) -> int {
+        const int blocks = t.chunks < 2048 ? (int)t.chunks : 2048;
         grad_scale_kernel<<<blocks, 256, 0, ctx->stream>>>(t, part, n_part, (double)max_norm, any ? nullptr : d_norm);
         TF_HIP(hipGetLastError());
         any = true;
@@ -292,4 +375,135 @@ extern "C" int tfrec_grad_clip(tfrec_ctx *ctx, int n, const void *const *h_grads
         TF_HIP(hipGetLastError());
     }
     return TFREC_OK;
+}
+
+static int finish_norm(tfrec_ctx *ctx, int n_part, float *d_norm)
+{
+    grad_norm_kernel<<<1, 256, 0, ctx->stream>>>((const double *)ctx->d_small, n_part, d_norm);
+    TF_HIP(hipGetLastError());
+    return TFREC_OK;
+}
+
+static int check_bound(float max_norm, const float *d_norm)
+{
+    TF_REQUIRE(max_norm > 0.f && max_norm < INFINITY, TFREC_EINVAL, "max_norm must be positive and finite, got %g", (double)max_norm);
+    TF_REQUIRE(((uintptr_t)d_norm & 3u) == 0, TFREC_EINVAL, "misaligned output");
+    return TFREC_OK;
+}
+
+extern "C" int tfrec_grad_norm(tfrec_ctx *ctx, int n, const void *const *h_grads, const int64_t *h_counts, const int *h_dtypes, float *d_norm)
+{
+    TF_TRY(check_grads(n, h_grads, h_counts, h_dtypes));
+    TF_REQUIRE(d_norm && ((uintptr_t)d_norm & 3u) == 0, TFREC_EINVAL, "null or misaligned output");
+    TF_TRY(tfrec_ctx_enter(ctx));
+    auto each = [&](auto &&f) -> int { return for_tables(n, h_grads, nullptr, h_counts, h_dtypes, f); };
+    int64_t most = 0;
+    TF_TRY(each([&](const GradTable &t) -> int { most = t.chunks > most ? t.chunks : most; return TFREC_OK; }));
+    int n_part = 0;
+    TF_TRY(run_norm(ctx, most, each, &n_part));
+    return finish_norm(ctx, n_part, d_norm);
+}
+
+extern "C" int tfrec_grad_clip(tfrec_ctx *ctx, int n, const void *const *h_grads, void *const *h_out, const int64_t *h_counts,
+                               const int *h_dtypes, float max_norm, float *d_norm)
+{
+    TF_TRY(check_grads(n, h_grads, h_counts, h_dtypes));
+    TF_TRY(check_bound(max_norm, d_norm));
+    TF_TRY(check_outputs(n, h_grads, h_out, h_counts, h_dtypes));
+    TF_TRY(tfrec_ctx_enter(ctx));
+    auto each = [&](auto &&f) -> int { return for_tables(n, h_grads, h_out, h_counts, h_dtypes, f); };
+    int64_t most = 0;
+    int tables = 0;
+    TF_TRY(each([&](const GradTable &t) -> int { most = t.chunks > most ? t.chunks : most; ++tables; return TFREC_OK; }));
+    return run_clip(ctx, most, tables, each, max_norm, d_norm);
+}
+
+// ------------------------------------------------------------------------------------------
+// kept lists
+// ------------------------------------------------------------------------------------------
+struct tfrec_grads {
+    GradChunk *d_chunks = nullptr;
+    int64_t chunks = 0;
+    int device = 0;
+};
+
+extern "C" int tfrec_grads_create(tfrec_ctx *ctx, int n, const void *const *h_grads, void *const *h_out, const int64_t *h_counts,
+                                  const int *h_dtypes, tfrec_grads **out)
+{
+    TF_REQUIRE(out != nullptr, TFREC_EINVAL, "out is null");
+    *out = nullptr;
+    TF_TRY(check_grads(n, h_grads, h_counts, h_dtypes));
+    TF_TRY(check_outputs(n, h_grads, h_out, h_counts, h_dtypes));
+    TF_TRY(tfrec_ctx_enter(ctx));
+    int64_t chunks = 0;
+    for (int i = 0; i < n; ++i) chunks += (h_counts[i] + GRAD_CHUNK - 1) / GRAD_CHUNK;
+    tfrec_grads *g = new (std::nothrow) tfrec_grads();
+    GradChunk *h = new (std::nothrow) GradChunk[(size_t)chunks + 1];
+    if (!g || !h) {
+        delete g;
+        delete[] h;
+        tfrec_set_error("host allocation failed");
+        return TFREC_ENOMEM;
+    }
+    int64_t c = 0;
+    for (int i = 0; i < n; ++i)
+        for (int64_t at = 0; at < h_counts[i]; at += GRAD_CHUNK) {
+            const size_t es = dt_size(h_dtypes[i]);
+            const int64_t left = h_counts[i] - at;
+            h[c++] = GradChunk{(const char *)h_grads[i] + at * es, (char *)h_out[i] + at * es, (int32_t)(left < GRAD_CHUNK ? left : GRAD_CHUNK), h_dtypes[i], 0};
+        }
+    g->chunks = chunks;
+    g->device = ctx->device;
+    hipError_t e = hipMalloc((void **)&g->d_chunks, sizeof(GradChunk) * (size_t)(chunks > 0 ? chunks : 1));
+    if (e != hipSuccess) g->d_chunks = nullptr;
+    if (e == hipSuccess && chunks) e = hipMemcpyAsync(g->d_chunks, h, sizeof(GradChunk) * (size_t)chunks, hipMemcpyHostToDevice, ctx->stream);
+    if (e == hipSuccess) e = hipStreamSynchronize(ctx->stream);
+    delete[] h;
+    if (e != hipSuccess) {
+        const int code = g->d_chunks ? TFREC_EHIP : TFREC_ENOMEM;
+        if (g->d_chunks) (void)hipFree(g->d_chunks);
+        delete g;
+        tfrec_set_error("the list of %lld chunks could not be stored: %s", (long long)chunks, hipGetErrorString(e));
+        return code;
+    }
+    *out = g;
+    return TFREC_OK;
+}
+
+extern "C" int tfrec_grads_destroy(tfrec_ctx *ctx, tfrec_grads *g)
+{
+    if (!g) return TFREC_OK;
+    (void)hipSetDevice(g->device);
+    if (ctx) (void)hipStreamSynchronize(ctx->stream);
+    else (void)hipDeviceSynchronize();
+    if (g->d_chunks) (void)hipFree(g->d_chunks);
+    delete g;
+    return TFREC_OK;
+}
+
+static int check_list(tfrec_ctx *ctx, const tfrec_grads *g)
+{
+    TF_REQUIRE(g->device == ctx->device, TFREC_EINVAL, "the list was made on device %d, the context is on device %d", g->device, ctx->device);
+    return TFREC_OK;
+}
+
+extern "C" int tfrec_grads_norm(tfrec_ctx *ctx, const tfrec_grads *g, float *d_norm)
+{
+    TF_REQUIRE(g != nullptr, TFREC_EINVAL, "null list");
+    TF_REQUIRE(d_norm && ((uintptr_t)d_norm & 3u) == 0, TFREC_EINVAL, "null or misaligned output");
+    TF_TRY(tfrec_ctx_enter(ctx));
+    TF_TRY(check_list(ctx, g));
+    int n_part = 0;
+    TF_TRY(run_norm(ctx, g->chunks, [&](auto &&f) -> int { return f(GradListed{g->d_chunks, g->chunks}); }, &n_part));
+    return finish_norm(ctx, n_part, d_norm);
+}
+
+extern "C" int tfrec_grads_clip(tfrec_ctx *ctx, const tfrec_grads *g, float max_norm, float *d_norm)
+{
+    TF_REQUIRE(g != nullptr, TFREC_EINVAL, "null list");
+    TF_TRY(check_bound(max_norm, d_norm));
+    TF_TRY(tfrec_ctx_enter(ctx));
+    TF_TRY(check_list(ctx, g));
+    if (g->chunks == 0 && !d_norm) return TFREC_OK;
+    return run_clip(ctx, g->chunks, 1, [&](auto &&f) -> int { return f(GradListed{g->d_chunks, g->chunks}); }, max_norm, d_norm);
 }

@@ -137,38 +137,54 @@ class QuantRows:
         return self.shape[0]
 
 
+def _grad_arrays(dev, grads, out):
+    """Host arrays (n, gradients, outputs, lengths, types) of a call on gradient tensors, types and devices checked."""
+    grads = list(grads)
+    out = None if out is None else list(out)
+    n = len(grads)
+    if out is not None and len(out) != n:
+        raise ValueError("%d outputs for %d gradients" % (len(out), n))
+    sizes = [_numel(g) for g in grads]
+    types = [_dt(g) for g in grads]
+    at = [_ptr_on(dev, g) for g in grads]
+    to = at
+    if out is not None:
+        for i, o in enumerate(out):
+            if _numel(o) != sizes[i] or _dt(o) != types[i]:
+                raise ValueError("output %d has another type or size than its gradient" % i)
+        to = [_ptr_on(dev, o) for o in out]
+    m = max(n, 1)
+    return n, (C.c_void_p * m)(*at), (C.c_void_p * m)(*to), (C.c_int64 * m)(*sizes), (C.c_int * m)(*types)
+
+
 class GradList:
     """Gradient tensors (float32, bfloat16 or float16, contiguous, any shape) and, optionally, the tensors their scaled
-    values go to (same types and sizes; default: in place), checked once: a program makes one for its gradient buffers and
-    passes it to every ``grad_norm`` / ``clip_grads``.  It keeps the tensors alive."""
+    values go to (same types and sizes; default: in place), checked once and laid out on the GPU: a program makes one for
+    its gradient buffers and passes it to every ``grad_norm`` / ``clip_grads``.  It keeps the tensors alive."""
 
     def __init__(self, dev, grads, out=None):
-        self.dev = dev
+        self.dev, self.h = dev, None
         self.grads = list(grads)
         self.out = self.grads if out is None else list(out)
-        n = len(self.grads)
-        if len(self.out) != n:
-            raise ValueError("%d outputs for %d gradients" % (len(self.out), n))
-        sizes, types, at, to = [], [], [], []
-        for g in self.grads:
-            sizes.append(_numel(g))
-            types.append(_dt(g))
-            at.append(_ptr_on(dev, g))
-        if out is None:
-            to = at
-        else:
-            for i, o in enumerate(self.out):
-                if _numel(o) != sizes[i] or _dt(o) != types[i]:
-                    raise ValueError("output %d has another type or size than its gradient" % i)
-                to.append(_ptr_on(dev, o))
-        self.n = n
-        self.c_grads = (C.c_void_p * max(n, 1))(*at)
-        self.c_out = (C.c_void_p * max(n, 1))(*to)
-        self.c_counts = (C.c_int64 * max(n, 1))(*sizes)
-        self.c_types = (C.c_int * max(n, 1))(*types)
+        n, at, to, sizes, types = _grad_arrays(dev, self.grads, None if out is None else self.out)
+        h = C.c_void_p()
+        _lib.check(dev.lib.tfrec_grads_create(dev.h, n, at, to, sizes, types, C.byref(h)))
+        self.h = h.value
 
     def __len__(self):
-        return self.n
+        return len(self.grads)
+
+    def close(self):
+        """Frees the list (the tensors are the caller's); also after the Device was closed."""
+        if self.h:
+            h, self.h = self.h, None
+            self.dev.lib.tfrec_grads_destroy(self.dev.h, h)
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
 
 
 _DT = {"float32": _lib.DT_F32, "bfloat16": _lib.DT_BF16, "float16": _lib.DT_F16}
@@ -504,24 +520,28 @@ class Device:
 
     def grad_norm(self, grads, norm=None):
         """Global l2 norm over the tensors (a sequence or a ``GradList``), float32 [1] on the GPU."""
-        g = grads if isinstance(grads, GradList) else GradList(self, grads)
         norm = norm if norm is not None else self.empty(1, np.float32)
-        _lib.check(self.lib.tfrec_grad_norm(self.h, g.n, g.c_grads, g.c_counts, g.c_types, _vector(self, norm, 1, "float32", "norm")))
+        to = _vector(self, norm, 1, "float32", "norm")
+        if isinstance(grads, GradList):
+            _lib.check(self.lib.tfrec_grads_norm(self.h, grads.h, to))
+        else:
+            n, at, _, sizes, types = _grad_arrays(self, grads, None)
+            _lib.check(self.lib.tfrec_grad_norm(self.h, n, at, sizes, types, to))
         return norm
 
     def clip_grads(self, grads, max_norm, out=None, norm=None):
         """Scales every tensor by ``max_norm / max(norm, max_norm)``, norm = the global l2 norm over all of them: in place, or
         into ``out`` (a sequence of tensors; with a ``GradList`` the list's own outputs).  Returns the norm before scaling,
         float32 [1] on the GPU.  A norm that is not finite makes every value NaN."""
+        norm = norm if norm is not None else self.empty(1, np.float32)
+        to = _vector(self, norm, 1, "float32", "norm")
         if isinstance(grads, GradList):
             if out is not None:
                 raise ValueError("a GradList has its outputs already")
-            g = grads
+            _lib.check(self.lib.tfrec_grads_clip(self.h, grads.h, float(max_norm), to))
         else:
-            g = GradList(self, grads, out)
-        norm = norm if norm is not None else self.empty(1, np.float32)
-        _lib.check(self.lib.tfrec_grad_clip(self.h, g.n, g.c_grads, g.c_out, g.c_counts, g.c_types, float(max_norm),
-                                            _vector(self, norm, 1, "float32", "norm")))
+            n, at, dst, sizes, types = _grad_arrays(self, grads, out)
+            _lib.check(self.lib.tfrec_grad_clip(self.h, n, at, dst, sizes, types, float(max_norm), to))
         return norm
 
     # -- 8-bit rows -------------------------------------------------------------------------

@@ -21,15 +21,16 @@ class FoldOutEvaluator(AbstractEvaluator):
 
     Beside the reference's arguments (evaluator/evaluator.py:20): ``score_dtype`` "f32" (scores bit for bit the
     float32 fused-multiply-add chain; the default) or "bf16" (factors rounded to bfloat16, float32 accumulation: the
-    fast matrix-core path); ``metric_sum`` "reference" (per-user float32 curves summed sequentially in user order on
+    fast matrix-core path) or "i8" (every factor row in 8-bit integers with a scale of its own, exact integer sums: what
+    ``Device.score_topk_i8`` scores); ``metric_sum`` "reference" (per-user float32 curves summed sequentially in user order on
     the host, bit for bit evaluate.h:40-92; the default) or "float64" (sums formed on the device in float64, no
     per-user table: means agree with the reference's to about 1e-6 relative)."""
 
     @typeassert(train_matrix=csr_matrix, test_matrix=csr_matrix, top_k=int)
     def __init__(self, train_matrix, test_matrix, top_k=50, score_dtype="f32", metric_sum="reference"):
         super(FoldOutEvaluator, self).__init__()
-        if score_dtype not in ("f32", "bf16"):
-            raise ValueError("score_dtype must be 'f32' or 'bf16'")
+        if score_dtype not in ("f32", "bf16", "i8"):
+            raise ValueError("score_dtype must be 'f32', 'bf16' or 'i8'")
         if metric_sum not in ("reference", "float64"):
             raise ValueError("metric_sum must be 'reference' or 'float64'")
         self.top_k = top_k
@@ -49,8 +50,8 @@ class FoldOutEvaluator(AbstractEvaluator):
 
     @property
     def score_mode(self):
-        from ..device import SCORE_BF16, SCORE_F32
-        return SCORE_BF16 if self.score_dtype == "bf16" else SCORE_F32
+        from ..device import SCORE_BF16, SCORE_F32, SCORE_I8
+        return {"f32": SCORE_F32, "bf16": SCORE_BF16, "i8": SCORE_I8}[self.score_dtype]
 
     def metrics_info(self):
         return ", ".join("%s@1:1:%d" % (m, self.top_k) for m in ("Precision", "Recall", "MAP", "NDCG", "MRR"))

@@ -11,7 +11,7 @@ import numpy as np
 from ..data import DataIterator, DeviceEpochSampler
 from ..device import Device
 from ..utils import csr_to_user_dict, load_params, random_choice
-from .BPR import BPR, _Quiet, process_group
+from .BPR import BPR, _Quiet, clip_norm_of, process_group
 from .base import AbstractRecommender, MatrixFactorization
 
 
@@ -19,6 +19,8 @@ class APR(AbstractRecommender):
     def __init__(self, sess, config, dataset, evaluator):
         super(APR, self).__init__(sess, config, dataset, evaluator)
         self.config = config
+        if clip_norm_of(config):
+            raise ValueError("clip_norm is offered by BPR and DNSBPR")
         train_matrix = dataset.train_matrix
         self.users_num, self.items_num = train_matrix.shape
         self.factors_num = config["factors_num"]

@@ -3,7 +3,7 @@
 Keys read from the configuration: the reference's (factors_num, lr, reg, epochs, batch_size, model/BPR.py:22-26)
 and, all optional with the reference's behaviour as the default: ``sampler`` (host | device), ``seed``,
 ``item_mode`` (auto | dense | sharded: how the item table is laid out over several GPUs), ``checkpoint_file``,
-``resume``.  Started as one process per GPU (run_model.py with ``devices = N``, or torchrun) the same class trains
+``resume``, ``clip_norm`` (a bound on the l2 norm of a batch's whole gradient, 0 = none; one GPU).  Started as one process per GPU (run_model.py with ``devices = N``, or torchrun) the same class trains
 on row-sharded tables (tfrec_amd/sharded.py): rank 0 logs, every rank steps.
 """
 import numpy as np
@@ -25,6 +25,14 @@ def process_group():
     return 0, 1
 
 
+def clip_norm_of(config):
+    """The configuration's ``clip_norm``: a positive number, or 0 (the default) for steps without a bound."""
+    value = config["clip_norm"] if "clip_norm" in config else 0
+    if isinstance(value, bool) or not isinstance(value, (int, float)) or not 0 <= value < float("inf"):
+        raise ValueError("clip_norm must be a positive number, or 0 for none, got %r" % (value,))
+    return float(value)
+
+
 class _Quiet:
     """Logger of the ranks other than 0."""
 
@@ -40,6 +48,8 @@ class BPR(AbstractRecommender):
     def __init__(self, sess, config, dataset, evaluator):
         super(BPR, self).__init__(sess, config, dataset, evaluator)
         self.config = config
+        self.clip_norm = clip_norm_of(config)
+        self._grads = None
         train_matrix = dataset.train_matrix
         self.users_num, self.items_num = train_matrix.shape
         self.factors_num = config["factors_num"]
@@ -59,6 +69,8 @@ class BPR(AbstractRecommender):
         self.sharded = self.world > 1 or bool(config.get("force_sharded", False))
         self._ut = None
         if self.sharded:
+            if self.clip_norm:
+                raise ValueError("clip_norm is a single-GPU feature")
             self._init_sharded(train_matrix)
             return
         self.user_pos_train = csr_to_user_dict(train_matrix)
@@ -131,6 +143,9 @@ class BPR(AbstractRecommender):
         dev = self.sess
         P, Q, b = self.mf.device_parameters()
         n = len(bounds) - 1
+        if self.clip_norm:
+            self._run_clipped_steps(du, dp, dn, bounds)
+            return
         if self.batch_size < self.VERSIONED_FROM:
             for k in range(n):
                 lo, hi = bounds[k], bounds[k + 1]
@@ -153,6 +168,23 @@ class BPR(AbstractRecommender):
         finally:
             ut.flatten()            # P is complete again for the evaluation (or whatever else reads it next)
             dev.synchronize()
+
+    def _run_clipped_steps(self, du, dp, dn, bounds):
+        """Steps whose whole gradient (P, Q and b together) is scaled to a norm of at most ``clip_norm`` first.  Where no
+        batch reaches the bound the tables end up bit for bit as without it."""
+        dev = self.sess
+        tables = self.mf.device_parameters()
+        if self._grads is None:
+            grads = [dev.empty(t.shape, np.float32) for t in tables]
+            self._grads = dev.grad_list(grads), dev.empty(1, np.float32)
+        grads, norm = self._grads
+        for k in range(len(bounds) - 1):
+            lo, hi = bounds[k], bounds[k + 1]
+            dev.bpr_grads(*tables, du.view(lo, hi), dp.view(lo, hi), dn.view(lo, hi), self.reg, *grads.grads)
+            dev.clip_grads(grads, self.clip_norm, norm=norm)
+            for table, grad in zip(tables, grads.grads):
+                dev.axpy(table, grad, -self.lr)
+        dev.synchronize()
 
     def _train_epoch(self, train_data):
         """One epoch of minibatch steps (model/BPR.py:68-72): the epoch's triples are uploaded once

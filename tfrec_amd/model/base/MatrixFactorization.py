@@ -37,9 +37,18 @@ class MatrixFactorization(object):
         self.dev.synchronize()
         return out.numpy()
 
-    def all_logits(self, users=None):
+    def all_logits(self, users=None, score_dtype="f32"):
         """Scores of the given users (or all) against all items (MatrixFactorization.py:34-46),
-        on the host: meant for small problems and debugging, not for the training path."""
+        on the host: meant for small problems and debugging, not for the training path.  ``score_dtype`` "i8": the
+        scores an evaluator with that setting ranks (rows in 8 bits, formed on the GPU)."""
+        if score_dtype == "i8":
+            rows = None if users is None else self.dev.array(np.asarray(users), np.int32)
+            scores = self.dev.matmul_i8(self.dev.quantize_rows(self.user_embeddings, rows=rows), self.dev.quantize_rows(self.item_embeddings),
+                                        bias=self.item_biases)
+            self.dev.synchronize()
+            return scores.numpy()
+        if score_dtype != "f32":
+            raise ValueError("score_dtype must be 'f32' or 'i8'")
         P, Q, b = self.parameters()
         rows = P if users is None else P[np.asarray(users)]
         return np.matmul(rows, Q.T) + b
