@@ -179,10 +179,13 @@ __global__ __launch_bounds__(1024) void grad_clip_small_kernel(Table t, double m
     uint4 held[GRAD_SMALL][2];                 // 8 values of each chunk: two packs of 4, or one of 8
     double s = 0.;
     const int n = (int)t.chunks;
+    GradChunk cs[GRAD_SMALL];                  // all looked up before the first is used: one wait, not one per chunk
+#pragma unroll
+    for (int k = 0; k < GRAD_SMALL; ++k) cs[k] = n ? t.get(k < n ? k : n - 1) : GradChunk{};
 #pragma unroll
     for (int k = 0; k < GRAD_SMALL; ++k) {
         if (k >= n) break;
-        const GradChunk c = t.get(k);
+        const GradChunk &c = cs[k];
         by_type(c, [&]<class T>(const T *x, T *) {
             constexpr int V = 16 / sizeof(T), R = 8 / V;
 #pragma unroll
@@ -200,7 +203,7 @@ __global__ __launch_bounds__(1024) void grad_clip_small_kernel(Table t, double m
 #pragma unroll
     for (int k = 0; k < GRAD_SMALL; ++k) {
         if (k >= n) break;
-        const GradChunk c = t.get(k);
+        const GradChunk &c = cs[k];
         by_type(c, [&]<class T>(const T *, T *) {
             constexpr int V = 16 / sizeof(T), R = 8 / V;
 #pragma unroll
@@ -217,7 +220,7 @@ __global__ __launch_bounds__(1024) void grad_clip_small_kernel(Table t, double m
 #pragma unroll
     for (int k = 0; k < GRAD_SMALL; ++k) {
         if (k >= n) break;
-        const GradChunk c = t.get(k);
+        const GradChunk &c = cs[k];
         if (f.nothing(c)) continue;
         by_type(c, [&]<class T>(const T *, T *y) {
             constexpr int V = 16 / sizeof(T), R = 8 / V;

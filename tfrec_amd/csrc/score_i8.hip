@@ -71,10 +71,10 @@ struct RowDot {
         if constexpr (LPI > 8) s += __builtin_amdgcn_mov_dpp(s, 0x140, 0xf, 0xf, true);      // mirror of the row
         return s;
     }
-    __device__ __forceinline__ float score(const ScoreI8Args &a, int acc, int64_t it) const
-    {
-        return add_rounded(scaled_sum(acc, sp, a.sq[a.item_lo + it]), a.b ? a.b[a.item_lo + it] : 0.f);
-    }
+    // an item's scale and bias, requested with its row
+    struct Scale { float sq, b; };
+    __device__ __forceinline__ Scale scale(const ScoreI8Args &a, int64_t it) const { return {a.sq[a.item_lo + it], a.b ? a.b[a.item_lo + it] : 0.f}; }
+    __device__ __forceinline__ float score(int acc, Scale s) const { return add_rounded(scaled_sum(acc, sp, s.sq), s.b); }
     // Of 256 positions scored together, thread t owns this one: after LPI steps of 256 / LPI positions every thread has one.
     static __device__ __forceinline__ int owned() { return (threadIdx.x % LPI) * (256 / LPI) + (threadIdx.x & 255) / LPI; }
 };
@@ -405,7 +405,8 @@ __device__ __forceinline__ void group_finish(GroupList<LIST> &g, const ScoreI8Ar
     const int lane = threadIdx.x, cnt = g.count;
     float tau;
     int kept;
-    if (cnt <= 256) kept = wave_compact<256>(g.list, cnt, 0, a.k, midx, mlo, mhi, g.sorted, lane, &tau);
+    if (cnt <= 128) kept = wave_compact<128>(g.list, cnt, 0, a.k, midx, mlo, mhi, g.sorted, lane, &tau);
+    else if (cnt <= 256) kept = wave_compact<256>(g.list, cnt, 0, a.k, midx, mlo, mhi, g.sorted, lane, &tau);
     else kept = wave_compact<LIST>(g.list, cnt, 0, a.k, midx, mlo, mhi, g.sorted, lane, &tau);
     for (int e = lane; e < a.k; e += 64) {
         const uint64_t key = e < kept ? g.sorted[e] : 0;
@@ -436,7 +437,7 @@ __global__ __launch_bounds__(NT) void pick_i8_kernel(MaxArgs m)
     __shared__ uint16_t slices[SLICES];
     __shared__ uint8_t train[SLICES];
     __shared__ int n_slices, n_units, n_cand;
-    __shared__ float slack;
+    __shared__ uint32_t slack;
     constexpr int V = SLICES / NT;
     const ScoreI8Args &a = m.s;
     const int tid = threadIdx.x;
@@ -476,13 +477,15 @@ __global__ __launch_bounds__(NT) void pick_i8_kernel(MaxArgs m)
     }
     for (int i = tid; i < SLICES; i += NT) train[i] = 0;
     if (tid == 0) { g.count = 0; n_slices = 0; n_units = 0; n_cand = 0; }
-    if (tid < 64) {
-        float w = 0.f;
-        for (int i = tid; i < m.splits; i += 64) w = fmaxf(w, m.slack[r * m.splits + i]);
-        for (int o = 32; o > 0; o >>= 1) w = fmaxf(w, __shfl_xor(w, o, 64));
-        if (tid == 0) slack = w;
-    }
+    if (tid == 0) slack = 0u;
     __syncthreads();
+    {
+        // (not negative: the order of the bits is the order of the values, and a maximum has no order of arrival)
+        float w = 0.f;
+        for (int i = tid; i < m.splits; i += NT) w = fmaxf(w, m.slack[r * m.splits + i]);
+        for (int o = 32; o > 0; o >>= 1) w = fmaxf(w, __shfl_xor(w, o, 64));
+        if ((tid & 63) == 0) atomicMax(&slack, __float_as_uint(w));
+    }
     // (an index of any other sign or size is another shard's item)
     auto mark = [&](int32_t id) {
         const int64_t i = id - id0;
@@ -499,7 +502,7 @@ __global__ __launch_bounds__(NT) void pick_i8_kernel(MaxArgs m)
     float T = -INFINITY;
     if (cut) {
         const float c = fminf(orderable_f32(cut), -LOWEST);
-        T = c - 2.1f * slack - fabsf(c) * 0x1p-19f;
+        T = c - 2.1f * __uint_as_float(slack) - fabsf(c) * 0x1p-19f;
         T = T > LOWEST ? T : -INFINITY;           // (also where T is not a number)
     }
 #pragma unroll
@@ -533,8 +536,16 @@ __global__ __launch_bounds__(NT) void pick_i8_kernel(MaxArgs m)
             const int c = n_cand;
             for (int c0 = 0; c0 < c * CELL; c0 += 256 * ROUNDS) {
                 int acc[ROUNDS];
+                int64_t own[ROUNDS];
+                typename RowDot<LPI>::Scale sc[ROUNDS];
                 if (tid < 256) {
                     uint4 q[ROUNDS][LPI];
+#pragma unroll
+                    for (int o = 0; o < ROUNDS; ++o) {
+                        const int i = c0 + 256 * o + RowDot<LPI>::owned();
+                        own[o] = i < c * CELL ? cell_item(cand[i / CELL], i % CELL) : a.n_items;
+                        sc[o] = dot.scale(a, own[o] < a.n_items ? own[o] : 0);
+                    }
 #pragma unroll
                     for (int o = 0; o < ROUNDS; ++o)
 #pragma unroll
@@ -556,13 +567,11 @@ __global__ __launch_bounds__(NT) void pick_i8_kernel(MaxArgs m)
                 for (int o = 0; o < ROUNDS; ++o) {
                     if (o > 0 && c0 + 256 * o >= c * CELL) break;
                     if (tid < 256) {
-                        const int i = c0 + 256 * o + RowDot<LPI>::owned();
-                        const int64_t it = i < c * CELL ? cell_item(cand[i / CELL], i % CELL) : a.n_items;
                         bool pass = false;
                         uint64_t k64 = 0;
-                        if (it < a.n_items) {
-                            const float v = dot.score(a, acc[o], it);
-                            k64 = make_key(v, (int32_t)(id0 + it));
+                        if (own[o] < a.n_items) {
+                            const float v = dot.score(acc[o], sc[o]);
+                            k64 = make_key(v, (int32_t)(id0 + own[o]));
                             pass = v > -INFINITY && k64 > g.kth;
                         }
                         group_append(g, pass, k64);
@@ -606,26 +615,37 @@ __global__ __launch_bounds__(256) void score_small_i8_kernel(ScoreI8Args a)
         }
     __syncthreads();
     uint32_t key[V];
+    constexpr int BATCH = LPI <= 4 ? 4 : (LPI == 8 ? 2 : 1);           // rounds of 256 items whose rows are requested together
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-        key[v] = 0;
-        if (256 * v >= n_items) continue;
-        uint4 q[LPI];
+    for (int v0 = 0; v0 < V; v0 += BATCH) {
 #pragma unroll
-        for (int j = 0; j < LPI; ++j) {
-            const int i = 256 * v + j * (256 / LPI) + tid / LPI;
-            q[j] = dot.load(a, i < n_items ? i : 0);
+        for (int o = 0; o < BATCH; ++o) key[v0 + o] = 0;
+        if (256 * v0 >= n_items) continue;
+        uint4 q[BATCH][LPI];
+        typename RowDot<LPI>::Scale sc[BATCH];
+#pragma unroll
+        for (int o = 0; o < BATCH; ++o) {
+            const int i = 256 * (v0 + o) + own;
+            sc[o] = dot.scale(a, i < n_items ? i : 0);
+#pragma unroll
+            for (int j = 0; j < LPI; ++j) {
+                const int it = 256 * (v0 + o) + j * (256 / LPI) + tid / LPI;
+                q[o][j] = dot.load(a, it < n_items ? it : 0);
+            }
         }
-        int acc = 0;
 #pragma unroll
-        for (int j = 0; j < LPI; ++j) {
-            const int s = dot.dot(q[j]);
-            if (tid % LPI == j) acc = s;
-        }
-        const int i = 256 * v + own;
-        if (i < n_items && !(train[i >> 5] >> (i & 31) & 1u)) {
-            const float s = dot.score(a, acc, i);
-            key[v] = s > -INFINITY ? f32_orderable(s) : 0u;
+        for (int o = 0; o < BATCH; ++o) {
+            int acc = 0;
+#pragma unroll
+            for (int j = 0; j < LPI; ++j) {
+                const int s = dot.dot(q[o][j]);
+                if (tid % LPI == j) acc = s;
+            }
+            const int i = 256 * (v0 + o) + own;
+            if (i < n_items && !(train[i >> 5] >> (i & 31) & 1u)) {
+                const float s = dot.score(acc, sc[o]);
+                key[v0 + o] = s > -INFINITY ? f32_orderable(s) : 0u;
+            }
         }
     }
     const uint32_t cut = rank_bound<256, V>(key, KEY_NONE, a.k, g);

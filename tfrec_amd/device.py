@@ -131,7 +131,18 @@ class QuantRows:
         self.q, self.scale, self.d = q, scale, d
         self.shape = (shape[0], d)
         self.ld = shape[1]
-        _ptr(q), _ptr(scale)            # device buffers, contiguous
+        # (the description of a matrix that stays where it is: looked up once, not at every call)
+        self.at = _ptr(q), _ptr(scale)
+        where = {_gpu_of(q), _gpu_of(scale)}
+        if len(where) != 1:
+            raise ValueError("q and scale are on different devices")
+        self.gpu = where.pop()
+
+    def on(self, dev):
+        """(address of q, address of scale), refused where they are not on ``dev``'s GPU."""
+        if self.gpu != dev.device:
+            raise ValueError("the 8-bit matrix is on %s, the context on GPU %d" % ("the host" if self.gpu is None else "GPU %d" % self.gpu, dev.device))
+        return self.at
 
     def __len__(self):
         return self.shape[0]
@@ -190,8 +201,22 @@ class GradList:
 _DT = {"float32": _lib.DT_F32, "bfloat16": _lib.DT_BF16, "float16": _lib.DT_F16}
 
 
+_names = {}             # numpy or torch dtype -> its name
+
+
 def _dtype_name(x):
-    return str(x.dtype).rsplit(".", 1)[-1]
+    name = _names.get(x.dtype)
+    if name is None:
+        name = _names[x.dtype] = str(x.dtype).rsplit(".", 1)[-1]
+    return name
+
+
+def _gpu_of(x):
+    """Ordinal of the GPU a buffer lives on; None for host memory."""
+    if isinstance(x, (DevArray, DevView)):
+        return x.dev.device
+    where = getattr(x, "device", None)
+    return where.index if where is not None and where.type == "cuda" else None
 
 
 def _dt(x):
@@ -211,12 +236,8 @@ def _numel(x):
 
 def _ptr_on(dev, x):
     """``_ptr`` of a buffer that has to live on ``dev``'s GPU."""
-    where = getattr(x, "device", None)
-    if where is not None and hasattr(x, "data_ptr"):
-        if where.type != "cuda" or where.index != dev.device:
-            raise ValueError("the tensor is on %s, the context on GPU %d" % (where, dev.device))
-    elif isinstance(x, (DevArray, DevView)) and x.dev.device != dev.device:
-        raise ValueError("the array is on GPU %d, the context on GPU %d" % (x.dev.device, dev.device))
+    if x is not None and not isinstance(x, int) and _gpu_of(x) != dev.device:
+        raise ValueError("the buffer is on %s, the context on GPU %d" % (getattr(x, "device", "another GPU"), dev.device))
     return _ptr(x)
 
 
@@ -555,8 +576,8 @@ class Device:
             out = QuantRows(self.empty((n, (d + 15) // 16 * 16), np.int8), self.empty(n, np.float32), d)
         if out.shape != (n, d):
             raise ValueError("out holds %s, need %s" % (out.shape, (n, d)))
-        _lib.check(self.lib.tfrec_quantize_rows_i8(self.h, xp, _dt(X), n_rows, ldx, d, _vector(self, rows, n, "int32", "rows"), n,
-                                                   _ptr_on(self, out.q), out.ld, _ptr_on(self, out.scale)))
+        q, scale = out.on(self)
+        _lib.check(self.lib.tfrec_quantize_rows_i8(self.h, xp, _dt(X), n_rows, ldx, d, _vector(self, rows, n, "int32", "rows"), n, q, out.ld, scale))
         return out
 
     def matmul_i8(self, A, B, bias=None, out=None):
@@ -569,8 +590,9 @@ class Device:
         if _shape(out) != (M, N):
             raise ValueError("out must be [%d, %d]" % (M, N))
         cp, ldc = _rows2d(self, out, "out")
-        _lib.check(self.lib.tfrec_matmul_i8(self.h, _ptr_on(self, A.q), A.ld, _ptr_on(self, A.scale), M, _ptr_on(self, B.q), B.ld,
-                                            _ptr_on(self, B.scale), N, K, _vector(self, bias, N, "float32", "bias"), cp, _dt(out), ldc))
+        aq, sa = A.on(self)
+        bq, sb = B.on(self)
+        _lib.check(self.lib.tfrec_matmul_i8(self.h, aq, A.ld, sa, M, bq, B.ld, sb, N, K, _vector(self, bias, N, "float32", "bias"), cp, _dt(out), ldc))
         return out
 
     def axpy(self, y, x, alpha, n=None):
@@ -653,9 +675,12 @@ class Device:
         if _shape(out_ids) != (n, k) or _dtype_name(out_ids) != "int32" or _shape(out_scores) != (n, k) or _dtype_name(out_scores) != "float32":
             raise ValueError("outputs must be int32 and float32 [%d, %d]" % (n, k))
         tp, ti = (train if train is not None else (None, None))
-        _lib.check(self.lib.tfrec_score_topk_i8(self.h, _ptr_on(self, P.q), P.ld, _ptr_on(self, P.scale), U, 1 if compact else 0, _ptr_on(self, Q.q),
-                                                Q.ld, _ptr_on(self, Q.scale), _vector(self, b, I, "float32", "b"), I, d, int(lo), int(hi),
-                                                _vector(self, eval_users, n, "int32", "eval_users"), n, _ptr(tp), _ptr(ti), k,
+        if train is not None and (_dtype_name(tp) != "int64" or _dtype_name(ti) != "int32" or (not compact and _shape(tp)[0] <= U)):
+            raise ValueError("train needs int64 row starts (one more than users) and int32 items")
+        pq, sp = P.on(self)
+        qq, sq = Q.on(self)
+        _lib.check(self.lib.tfrec_score_topk_i8(self.h, pq, P.ld, sp, U, 1 if compact else 0, qq, Q.ld, sq, _vector(self, b, I, "float32", "b"), I, d, int(lo), int(hi),
+                                                _vector(self, eval_users, n, "int32", "eval_users"), n, _ptr_on(self, tp), _ptr_on(self, ti), k,
                                                 _ptr_on(self, out_ids), _ptr_on(self, out_scores)))
         return out_ids, out_scores
 
