@@ -33,7 +33,7 @@ struct __attribute__((packed, aligned(sizeof(T)))) Values16 { T v[16]; };
 // LPR threads hold one row (a power of two up to 64: lanes of a wave; 256: the workgroup), CH runs of 16 columns each in
 // registers: one read of the row, one write of a quarter (half) as much.  CH = 0: rows too long for that are read twice,
 // the second time from the caches.
-// Bound by memory: 4096 x 8192 bf16 (96 MB in all) in the time the launch code below gives.
+// Bound by memory: 4096 x 8192 bf16 (96 MB in all) takes 30 us, 3.2 TB/s.
 template <class T, int LPR, int CH>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(const T *__restrict__ X, int64_t n_rows, int64_t ldx, int64_t d,
                                                             const int32_t *__restrict__ rows, int64_t n, int8_t *__restrict__ q, int64_t ldq,
@@ -165,6 +165,29 @@ extern "C" int tfrec_quantize_rows_i8(tfrec_ctx *ctx, const void *d_X, int x_dty
     return tfrec_quantize_rows(ctx, d_X, x_dtype, n_rows, ldx, d, d_rows, n, d_q, ldq, d_scale);
 }
 
+// The words W (8 or 16 bytes) as values of type T: one store, at T's alignment, or the first `room` values one by one.  (As a
+// vector type on purpose: the compiler takes the store of a struct apart and joins it with the other branch's.)
+template <class T, int W>
+__device__ __forceinline__ void store_values(T *to, const uint32_t (&w)[W], int64_t room)
+{
+    typedef uint32_t Words __attribute__((ext_vector_type(W), aligned(sizeof(T)), may_alias));
+    struct All { T v[4 * W / sizeof(T)]; };
+    if (room >= (int64_t)(4 * W / sizeof(T))) {
+        Words o;
+#pragma unroll
+        for (int i = 0; i < W; ++i) o[i] = w[i];
+        *reinterpret_cast<Words *>(to) = o;
+    } else {
+        struct In { uint32_t w[W]; } in;
+#pragma unroll
+        for (int i = 0; i < W; ++i) in.w[i] = w[i];
+        const All all = __builtin_bit_cast(All, in);
+#pragma unroll
+        for (int x = 0; x < (int)(4 * W / sizeof(T)); ++x)
+            if (x < room) to[x] = all.v[x];
+    }
+}
+
 // ------------------------------------------------------------------------------------------
 // product
 // ------------------------------------------------------------------------------------------
@@ -259,16 +282,15 @@ __global__ __launch_bounds__(64 * KW) void matmul_i8_rows_kernel(MatmulArgs a)
         if (m >= a.M) continue;
         const float sa = a.sa[m];
         T *to = reinterpret_cast<T *>(a.C) + m * a.ldc + n;
-        struct __attribute__((packed, aligned(sizeof(T)))) Four { T v[4]; } o;
+        struct Four { T v[4]; } o;
+        struct Words { uint32_t w[sizeof(T)]; };
 #pragma unroll
         for (int j = 0; j < 4; ++j) o.v[j] = (T)output(a, acc[t][j], sa, sb[j], bias[j]);
-        if (n + 4 <= a.N) *reinterpret_cast<Four *>(to) = o;
-        else
-            for (int j = 0; j < 4; ++j)
-                if (n + j < a.N) to[j] = o.v[j];
+        store_values(to, __builtin_bit_cast(Words, o).w, a.N - n);
     }
 }
 
+// ---- short rows: bound by the stores of C ------------------------------------------------------------------------------
 // 128 x 128 of C per workgroup, 64 x 64 per wave in four 32 x 32 blocks of v_mfma_i32_32x32x32_i8.  Tiles of 64 columns go
 // through LDS (two buffers; rows of 64 bytes, the chunk position XORed with the row so that fragment reads spread over
 // the banks).  Operand layout of the instruction: lane l holds 16 bytes of row l & 31, columns 16 (l >> 5) .. + 16;
@@ -278,11 +300,21 @@ __global__ __launch_bounds__(256) void matmul_i8_kernel(MatmulArgs a)
 {
     constexpr int BM = 128, BN = 128, KB = 64;
     __shared__ __align__(16) char lds[2][(BM + BN) * KB];
+    __shared__ float scale_a[BM];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int r = lane & 31, h = lane >> 5;
     const int64_t n_tiles = (a.N + BN - 1) / BN;
     const int64_t m0 = (int64_t)(blockIdx.x / n_tiles) * BM, n0 = (int64_t)(blockIdx.x % n_tiles) * BN;
     const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
+    // the scales and biases are requested first: they are here when the products are done
+    if (tid < BM) scale_a[tid] = a.sa[m0 + tid < a.M ? m0 + tid : a.M - 1];
+    float sb[2], bias[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int64_t n = n0 + wn + 32 * j + r, nc = n < a.N ? n : a.N - 1;
+        sb[j] = a.sb[nc];
+        bias[j] = a.bias ? a.bias[nc] : 0.f;
+    }
     i32x16 acc[2][2] = {};
     uint4 st[4];
     auto load = [&](int64_t kt) {
@@ -330,39 +362,59 @@ __global__ __launch_bounds__(256) void matmul_i8_kernel(MatmulArgs a)
         if (kt + 1 < steps) put(buf ^ 1);
         __syncthreads();
     }
+    // C through LDS, 16 rows of a wave's 64 columns at a time (rows padded by 16 bytes): stores of 16 bytes a lane that
+    // cover whole 128- or 256-byte pieces of C's rows
+    constexpr int PITCH = 64 * sizeof(T) + 16, LANES = 64 * sizeof(T) / 16, PER = 16 / sizeof(T);
+    char *mine = lds[0] + wave * 16 * PITCH;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const int64_t n = n0 + wn + 32 * j + r;
-        if (n >= a.N) continue;
-        const float sb = a.sb[n], bias = a.bias ? a.bias[n] : 0.f;
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int half = 0; half < 2; ++half) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int64_t m = m0 + wm + 32 * i + (e & 3) + 8 * (e >> 2) + 4 * h;
-                if (m < a.M) {
-                    reinterpret_cast<T *>(a.C)[m * a.ldc + n] = (T)output(a, acc[i][j][e], a.sa[m], sb, bias);
-                }
+            for (int e = 8 * half; e < 8 * half + 8; ++e) {
+                const int row = (e & 3) + 8 * (e >> 2) + 4 * h;
+                const float sa = scale_a[wm + 32 * i + row];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) *reinterpret_cast<T *>(mine + (row & 15) * PITCH + (32 * j + r) * sizeof(T)) = (T)output(a, acc[i][j][e], sa, sb[j], bias[j]);
             }
-    }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int q = 0; q < 16 * LANES / 64; ++q) {
+                const int row = (64 * q + lane) / LANES, col = (64 * q + lane) % LANES * PER;
+                const int64_t m = m0 + wm + 32 * i + 16 * half + row, n = n0 + wn + col;
+                const uint4 v = *reinterpret_cast<const uint4 *>(mine + row * PITCH + col * sizeof(T));
+                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                if (m < a.M) store_values(reinterpret_cast<T *>(a.C) + m * a.ldc + n, w, a.N - n);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+        }
 }
 
-// ---- large products: 256 x 256 of C per workgroup of eight waves, 128 x 64 per wave ------------------------------------
-// Bound by the matrix cores.  A step takes 128 columns: 32 matrix instructions of 32 x 32 x 32 a wave, two waves a SIMD.
-// Rows go from memory straight into LDS (global_load_lds_dwordx4: one kilobyte, eight rows, per instruction and wave), two
-// buffers of 64 KB: the next step's loads are issued among this step's products.  The LDS image has no row padding; position
+// ---- large products: WM x WN waves, FM x FN blocks of 32 x 32 of C per wave ----------------------------------------------
+// Bound by the matrix cores.  256 x 256 of C per workgroup (2 x 4 waves of 4 x 2 blocks, two waves a SIMD), or 128 x 128
+// (2 x 2 waves of 2 x 2 blocks) where the larger tiles are too few for the chip.  A step takes 128 columns: 4 FM FN matrix
+// instructions a wave.  Rows go from memory straight into LDS (global_load_lds_dwordx4: one kilobyte, eight rows, per
+// instruction and wave), two buffers: the next step's loads are issued among this step's products.  The LDS image has no row padding; position
 // c of row r holds the row's chunk c ^ (r & 7), so that fragment reads spread over the banks (the swizzle is on the source
 // address).  Rows past the ends of A and B read the last row, columns past K are masked out of A's fragments in the last
 // step.  C goes out through LDS, so that stores cover whole 128-byte pieces of its rows.
 template <class T>
 using global_ptr = __attribute__((address_space(1))) T *;
 
-static constexpr int BIG_LDS = 131072 + 1024;      // two buffers, and A's 256 scales
+template <int WM, int WN, int FM, int FN>
+struct BigGeom {
+    static constexpr int NW = WM * WN, SIDE = 32 * FM * WM, KB = 128, HALF = SIDE * KB, BUF = 2 * HALF;
+    static_assert(SIDE == 32 * FN * WN && SIDE / 8 == 4 * NW && FN == 2 && 2 * BUF / NW == 16384, "tiles are square, four loads a wave and side, 64 columns a wave");
+    static constexpr int LDS = 2 * BUF + SIDE * 4;     // two buffers, and A's scales
+};
 
-template <class T>
-__global__ __launch_bounds__(512) void matmul_i8_big_kernel(MatmulArgs a, int tiles_m, int tiles_n)
+template <class T, int WM, int WN, int FM, int FN>
+__global__ __launch_bounds__((64 * WM * WN)) void matmul_i8_big_kernel(MatmulArgs a, int tiles_m, int tiles_n)
 {
-    constexpr int KB = 128, HALF = 256 * KB, BUF = 2 * HALF;
+    using G = BigGeom<WM, WN, FM, FN>;
+    constexpr int KB = G::KB, HALF = G::HALF, BUF = G::BUF, NW = G::NW, SIDE = G::SIDE;
     extern __shared__ __align__(16) char lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 31, h = lane >> 5;
     // consecutive workgroups go to the 8 XCDs in turn: each XCD takes one run of tiles, four tiles of A rows at a time, so
@@ -372,31 +424,31 @@ __global__ __launch_bounds__(512) void matmul_i8_big_kernel(MatmulArgs a, int ti
     if (t >= tiles || (int)(blockIdx.x / 8) >= per) return;
     const int band = t / (4 * tiles_n), in_band = t - band * 4 * tiles_n;
     const int band_m = tiles_m - 4 * band < 4 ? tiles_m - 4 * band : 4;
-    const int64_t m0 = (int64_t)(4 * band + in_band % band_m) * 256, n0 = (int64_t)(in_band / band_m) * 256;
+    const int64_t m0 = (int64_t)(4 * band + in_band % band_m) * SIDE, n0 = (int64_t)(in_band / band_m) * SIDE;
 
-    // this wave's rows of a step: 8 * (8 i + wave) + lane / 8 of A and of B, i = 0..3
+    // this wave's rows of a step: 8 * (NW i + wave) + lane / 8 of A and of B, i = 0..3
     const int chunk = ((lane & 7) ^ (lane >> 3)) * 16;
     global_ptr<const char> src[8];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const int64_t row = 8 * (8 * i + wave) + (lane >> 3);
+        const int64_t row = 8 * (NW * i + wave) + (lane >> 3);
         src[i] = (global_ptr<const char>)(const char *)(a.A + (m0 + row < a.M ? m0 + row : a.M - 1) * a.lda);
         src[4 + i] = (global_ptr<const char>)(const char *)(a.B + (n0 + row < a.N ? n0 + row : a.N - 1) * a.ldb);
     }
     float *scale_a = reinterpret_cast<float *>(lds + 2 * BUF);
-    if (tid < 256) scale_a[tid] = a.sa[m0 + tid < a.M ? m0 + tid : a.M - 1];
+    if (tid < SIDE) scale_a[tid] = a.sa[m0 + tid < a.M ? m0 + tid : a.M - 1];
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
     auto request = [&](int64_t k0, int buf, int i) {
         const int64_t k = k0 + chunk;
         const global_ptr<const char> from = src[i] + (k < a.K ? k : 0);
-        const uint32_t to = __builtin_amdgcn_readfirstlane(lds0 + (uint32_t)(buf * BUF + (i >> 2) * HALF + (8 * (i & 3) + wave) * 1024));
+        const uint32_t to = __builtin_amdgcn_readfirstlane(lds0 + (uint32_t)(buf * BUF + (i >> 2) * HALF + (NW * (i & 3) + wave) * 1024));
         asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(to) : "memory", "m0");
     };
-    const int wm = (wave >> 2) * 128, wn = (wave & 3) * 64;
+    const int wm = wave / WN * (32 * FM), wn = wave % WN * (32 * FN);
     int off[KB / 32];
 #pragma unroll
     for (int ks = 0; ks < KB / 32; ++ks) off[ks] = r * KB + (((2 * ks + h) ^ (r & 7)) * 16);
-    i32x16 acc[4][2] = {};
+    i32x16 acc[FM][FN] = {};
     const int64_t steps = (a.K + KB - 1) / KB;
 #pragma unroll
     for (int i = 0; i < 8; ++i) request(0, 0, i);
@@ -408,15 +460,15 @@ __global__ __launch_bounds__(512) void matmul_i8_big_kernel(MatmulArgs a, int ti
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         const char *A = lds + buf * BUF + wm * KB, *B = lds + buf * BUF + HALF + wn * KB;
-        i32x4 fa[2][4], fb[2][2];
+        i32x4 fa[2][FM], fb[2][FN];
         auto fragments = [&](int ks, int to) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) fa[to][i] = *reinterpret_cast<const i32x4 *>(A + off[ks] + 32 * i * KB);
+            for (int i = 0; i < FM; ++i) fa[to][i] = *reinterpret_cast<const i32x4 *>(A + off[ks] + 32 * i * KB);
 #pragma unroll
-            for (int j = 0; j < 2; ++j) fb[to][j] = *reinterpret_cast<const i32x4 *>(B + off[ks] + 32 * j * KB);
+            for (int j = 0; j < FN; ++j) fb[to][j] = *reinterpret_cast<const i32x4 *>(B + off[ks] + 32 * j * KB);
             if (last)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) fa[to][i] = __builtin_bit_cast(i32x4, keep_below(__builtin_bit_cast(uint4, fa[to][i]), s * KB + 32 * ks + 16 * h, a.K));
+                for (int i = 0; i < FM; ++i) fa[to][i] = __builtin_bit_cast(i32x4, keep_below(__builtin_bit_cast(uint4, fa[to][i]), s * KB + 32 * ks + 16 * h, a.K));
         };
         fragments(0, 0);
 #pragma unroll
@@ -427,49 +479,42 @@ __global__ __launch_bounds__(512) void matmul_i8_big_kernel(MatmulArgs a, int ti
                 request((s + 1) * KB, buf ^ 1, 2 * ks + 1);
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < FM; ++i)
 #pragma unroll
-                for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa[ks & 1][i], fb[ks & 1][j], acc[i][j], 0, 0, 0);
+                for (int j = 0; j < FN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa[ks & 1][i], fb[ks & 1][j], acc[i][j], 0, 0, 0);
         }
     }
     __syncthreads();
 
-    // C: a wave's 128 x 64 in pieces of 32 rows through its 16 KB of LDS (rows padded by 16 bytes)
+    // C: a wave's 32 FM x 64 in pieces of 32 rows through its 16 KB of LDS (rows padded by 16 bytes)
     constexpr int PITCH = 64 * sizeof(T) + 16, LANES = 64 * sizeof(T) / 16, PER = 16 / sizeof(T);
     static_assert(32 * PITCH <= 16384, "a wave's piece exceeds its LDS");
     char *mine = lds + wave * 16384;
-    float sb[2], bias[2];
+    float sb[FN], bias[FN];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < FN; ++j) {
         const int64_t n = n0 + wn + 32 * j + r, nc = n < a.N ? n : a.N - 1;
         sb[j] = a.sb[nc];
         bias[j] = a.bias ? a.bias[nc] : 0.f;
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < FM; ++i) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
             const int row = (e & 3) + 8 * (e >> 2) + 4 * h;
             const float sa = scale_a[wm + 32 * i + row];
 #pragma unroll
-            for (int j = 0; j < 2; ++j) *reinterpret_cast<T *>(mine + row * PITCH + (32 * j + r) * sizeof(T)) = (T)output(a, acc[i][j][e], sa, sb[j], bias[j]);
+            for (int j = 0; j < FN; ++j) *reinterpret_cast<T *>(mine + row * PITCH + (32 * j + r) * sizeof(T)) = (T)output(a, acc[i][j][e], sa, sb[j], bias[j]);
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
-        struct __attribute__((packed, aligned(sizeof(T)))) Piece { T v[PER]; };
 #pragma unroll
         for (int q = 0; q < 32 * LANES / 64; ++q) {
             const int row = (64 * q + lane) / LANES, col = (64 * q + lane) % LANES * PER;
             const int64_t m = m0 + wm + 32 * i + row, n = n0 + wn + col;
             const uint4 v = *reinterpret_cast<const uint4 *>(mine + row * PITCH + col * sizeof(T));
-            if (m < a.M) {
-                T *to = reinterpret_cast<T *>(a.C) + m * a.ldc + n;
-                const Piece p = __builtin_bit_cast(Piece, v);
-                if (n + PER <= a.N) *reinterpret_cast<Piece *>(to) = p;
-                else
-                    for (int x = 0; x < PER; ++x)
-                        if (n + x < a.N) to[x] = p.v[x];
-            }
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+            if (m < a.M) store_values(reinterpret_cast<T *>(a.C) + m * a.ldc + n, w, a.N - n);
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -477,20 +522,34 @@ __global__ __launch_bounds__(512) void matmul_i8_big_kernel(MatmulArgs a, int ti
     }
 }
 
-// Which kernel: the 256 x 256 tiles where they fill the chip and a row is long enough to repay their 128 KB of LDS (one
-// workgroup a CU); 128 x 128 tiles where those do, at short rows (C's stores bound them, several workgroups a CU overlap);
-// else 16 rows of B at a time, which gives small products workgroups enough.
+template <class T, int WM, int WN, int FM, int FN>
+static int launch_big(tfrec_ctx *ctx, const MatmulArgs &a)
+{
+    using G = BigGeom<WM, WN, FM, FN>;
+    const int64_t tm = (a.M + G::SIDE - 1) / G::SIDE, tn = (a.N + G::SIDE - 1) / G::SIDE, tiles = tm * tn;
+    TF_REQUIRE(tiles < (1ll << 28), TFREC_EUNSUP, "the product is too large for one launch");
+    static std::atomic<uint64_t> done{0};
+    TF_TRY(tfrec_raise_lds_limit(ctx, reinterpret_cast<const void *>(&matmul_i8_big_kernel<T, WM, WN, FM, FN>), G::LDS, done));
+    matmul_i8_big_kernel<T, WM, WN, FM, FN><<<(unsigned)((tiles + 7) / 8 * 8), 64 * G::NW, G::LDS, ctx->stream>>>(a, (int)tm, (int)tn);
+    TF_HIP(hipGetLastError());
+    return TFREC_OK;
+}
+
+// Which kernel (us, measured on both sides of each rule):
+//   256 x 256 tiles where they fill the chip and a row is long enough to repay 128 KB of LDS, one workgroup a CU
+//     (4096 x 8192 x 8192: 264; 128 x 128 tiles 330 at the same rows);
+//   128 x 128 tiles of the same kernel for 64 rows of A and more, once there are 32 of them: 512 x 4096 x 4096 27 against 69
+//     for 16 rows of B at a time, 256 x 4096 x 4096 22 / 37, 128 x 4096 x 4096 even, 333 x 555 x 7777 (15 tiles) 39 / 31;
+//   rows below 256 columns are bound by the stores of C, which the kernel with 33 KB of LDS and several workgroups a CU
+//     serves best: 2048 x 200000 x 64 in float32 310 (5.3 TB/s; a fill of C alone 240) against 454;
+//   16 rows of B at a time for everything else: small products get workgroups enough, few rows of A are bound by reading B.
 template <class T>
 static int launch_matmul(tfrec_ctx *ctx, const MatmulArgs &a)
 {
-    const int64_t big_m = (a.M + 255) / 256, big_n = (a.N + 255) / 256, mid = ((a.M + 127) / 128) * ((a.N + 127) / 128);
-    if (a.K >= 512 && big_m * big_n >= 160) {
-        TF_REQUIRE(big_m * big_n < (1ll << 28), TFREC_EUNSUP, "the product is too large for one launch");
-        static std::atomic<uint64_t> done{0};
-        TF_TRY(tfrec_raise_lds_limit(ctx, reinterpret_cast<const void *>(&matmul_i8_big_kernel<T>), BIG_LDS, done));
-        const int64_t tiles = big_m * big_n;
-        matmul_i8_big_kernel<T><<<(unsigned)((tiles + 7) / 8 * 8), 512, BIG_LDS, ctx->stream>>>(a, (int)big_m, (int)big_n);
-    } else if (a.M > 128 && mid >= 192) {
+    const int64_t big = ((a.M + 255) / 256) * ((a.N + 255) / 256), mid = ((a.M + 127) / 128) * ((a.N + 127) / 128);
+    if (a.K >= 512 && big >= 160) return launch_big<T, 2, 4, 4, 2>(ctx, a);
+    if (a.M > 64 && mid >= 32 && a.K >= 256) return launch_big<T, 2, 2, 2, 2>(ctx, a);
+    if (a.M > 64 && mid >= 192) {
         TF_REQUIRE(mid < (1ll << 31), TFREC_EUNSUP, "the product is too large for one launch");
         matmul_i8_kernel<T><<<(unsigned)mid, 256, 0, ctx->stream>>>(a);
     } else {
