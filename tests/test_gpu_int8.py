@@ -468,3 +468,96 @@ def test_captured_calls_replay_on_new_inputs(dev):
         assert all(torch.equal(x, y) for x, y in zip(got, (C, ids, sc)))
         dev.topk_dense(torch.randn(4000 * (i + 1), 64, generator=g, device="cuda"), 5)         # the workspace grows: the graph's block stays
         torch.cuda.synchronize()
+
+
+# --------------------------------------------------------------------------------------- the sides of the launch rules
+@pytest.mark.parametrize("out", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("M,N,K", [(65, 4099, 256), (500, 1101, 300), (513, 1030, 1000), (1000, 3301, 200), (129, 12700, 20), (2100, 4701, 600), (4100, 2561, 529)])
+def test_product_tiles(dev, M, N, K, out):
+    A, sa, B, sb, b = product_case(M + N + K, M, N, K, bias=K % 3 != 0)
+    check_product(dev, A, sa * np.float32(0.02), B, sb, b, out)
+
+
+def test_product_tiles_into_a_pitched_slice(dev):
+    """Every tile kernel into an output whose rows start off their 16 bytes; what lies around it stays."""
+    for M, N, K in ((1000, 3301, 200), (500, 1101, 300), (2100, 4701, 512), (70, 131, 64)):
+        A, sa, B, sb, b = product_case(M + K, M, N, K)
+        a, w = quant_rows(A, sa, K), quant_rows(B, sb, K)
+        for out in ("f32", "bf16"):
+            dt = {"f32": torch.float32, "bf16": torch.bfloat16}[out]
+            whole = torch.full((M + 2, N + 5), 7.0, dtype=dt, device="cuda")
+            dev.matmul_i8(a, w, bias=torch.from_numpy(b).cuda(), out=whole[1:-1, 3:-2])
+            want = torch.empty(M, N, dtype=dt, device="cuda")
+            dev.matmul_i8(a, w, bias=torch.from_numpy(b).cuda(), out=want)
+            dev.synchronize()
+            assert torch.equal(whole[1:-1, 3:-2], want)
+            whole[1:-1, 3:-2] = 7.0
+            assert bool((whole == 7.0).all())
+
+
+@pytest.mark.parametrize("n,I,d,k,train", [
+    (200, 6000, 100, 20, 10), (97, 4097, 128, 33, 5), (20, 8000, 128, 10, 3), (33, 9000, 200, 10, 5), (3, 120000, 64, 20, 30), (300, 120000, 20, 20, 30),
+    (40, 110000, 150, 5, 3), (260, 100001, 31, 113, 2)])
+def test_topk_sets_and_groups(dev, n, I, d, k, train):
+    case = topk_case(n + I + d + k, n, I, d, train)
+    check_topk(dev, case, np.arange(n)[::-1], k)
+
+
+@pytest.mark.parametrize("n,I", [(3, 110000), (300, 100000), (70, 5000)])
+def test_topk_of_large_groups_with_ties(dev, n, I):
+    """Scores that repeat, so that lists end among equals, train items among the best."""
+    rng = np.random.default_rng(I)
+    Pq, sp, Qq, sq, b, _ = topk_case(n, n, I, 16, 0)
+    Qq[:] = Qq[rng.integers(0, 40, I)]
+    sq[:] = np.float32(0.5)
+    b[:] = np.float32(0.25)
+    S = scores_f32(Pq, sp, Qq, sq, b)
+    masks = [np.sort(rng.choice(np.flatnonzero(S[u] == S[u].max()), 30, replace=False)) if u % 3 else np.zeros(0, np.int64) for u in range(n)]
+    check_topk(dev, (Pq, sp, Qq, sq, b, masks), np.arange(n), 20)
+
+
+@pytest.mark.parametrize("n,I", [(3, 900), (5, 120000), (200, 20000)])
+def test_topk_of_negative_scales(dev, n, I):
+    Pq, sp, Qq, sq, b, masks = topk_case(n, n, I, 40, 6)
+    rng = np.random.default_rng(1)
+    sp *= rng.choice([-1, 1], n).astype(np.float32)
+    sq *= rng.choice([-1, 1], I).astype(np.float32)
+    b *= np.float32(0.001)
+    check_topk(dev, (Pq, sp, Qq, sq, b, masks), np.arange(n), 25)
+
+
+@pytest.mark.parametrize("n,I", [(2, 100000), (300, 6000)])
+def test_captured_topk_with_scratch(dev, n, I):
+    """Two graphs of calls that take scratch: replays in turn on changed inputs, eager calls that need more scratch between."""
+    g = torch.Generator(device="cuda").manual_seed(n)
+    P = torch.randn(n, 48, generator=g, device="cuda")
+    Q = torch.randn(I, 48, generator=g, device="cuda")
+    p, q = dev.quantize_rows(P), dev.quantize_rows(Q)
+    users = torch.arange(n, dtype=torch.int32, device="cuda")
+    outs = [(torch.zeros(n, k, dtype=torch.int32, device="cuda"), torch.zeros(n, k, device="cuda")) for k in (7, 30)]
+
+    def step(i):
+        dev.score_topk_i8(p, q, None, users, (7, 30)[i], out_ids=outs[i][0], out_scores=outs[i][1])
+    step(0), step(1)
+    torch.cuda.synchronize()
+    graphs = []
+    for i in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i], stream=dev._torch_stream):
+            step(i)
+    for turn in range(3):
+        dev.quantize_rows(torch.randn(n, 48, generator=g, device="cuda"), out=p)
+        torch.cuda.synchronize()
+        for i in (0, 1):
+            graphs[i].replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for o in outs for t in o]
+        for o in outs:
+            o[0].zero_(), o[1].zero_()
+        step(0), step(1)
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(got, [t for o in outs for t in o]))
+        big = torch.randint(-127, 128, (5000 * (turn + 1), 64), dtype=torch.int8, device="cuda")
+        wide = quant_rows(big.cpu().numpy(), np.ones(len(big), np.float32), 64)
+        dev.score_topk_i8(wide, wide, None, torch.arange(600 * (turn + 1), dtype=torch.int32, device="cuda"), 10)
+        torch.cuda.synchronize()

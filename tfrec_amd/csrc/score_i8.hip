@@ -86,7 +86,7 @@ struct MaxArgs {
     ScoreI8Args s;
     float *bound;              // [n, pitch]: cells
     float *group_bound;        // [n, groups]: the largest bound of a group's 16 cells
-    float *slack;              // [n, splits]: 1.6 sp sq, the largest over a split
+    float *slack;              // [n, splits]: 1.6 |sp sq|, the largest over a split
     int64_t pitch;             // cells per user row: 16 per group of 8 blocks
     int64_t groups;            // groups of 8 blocks
     int64_t groups_per_split;
@@ -107,10 +107,13 @@ static constexpr float NO_SCORE = LOWEST * (1.f - 0x1p-19f);
 //     v = fma(fma(acc, sp, -1.5 * 2^23 * sp), sq, b).
 // Against the defined score e: the inner step is off by at most half an ulp of 1.5 * 2^23 sp (0.75 sp) and of the result
 // (2^-24 * 2^22 sp), the defined products by 2 * 2^-24 of theirs (0.5 sp sq at most), and both sums by half an ulp of what
-// they give: |v - e| <= 1.6 sp sq + 2^-22 |v|, plus a few steps of 2^-149.  A cell's bound is its largest v plus that
+// they give: |v - e| <= 1.6 |sp sq| + 2^-22 |v|, plus a few steps of 2^-149.  A cell's bound is its largest v plus that
 // (with 2^-21 for its own rounding), its best e at least the bound less twice that; the first term, which does not show in
 // the bound, is kept per user and slice of the items.
-// Scales above 2^50 could leave float32's range in one form and not in the other: users and blocks that have such scales
+// 4096 users, 200k items of 64 columns: 125 to 140 us (0.8 * 10^15 operations/s; the vector instructions alone need 75, the
+// matrix instructions 50, and without its stores it takes 100 to 105).  33 users, 2M items of 128 columns: 69 us, 3.9 TB/s, bound
+// by reading the table.
+// Scales above 2^50 (of either sign) could leave float32's range in one form and not in the other: users and blocks that have such scales
 // take the definition itself.
 template <int KS, int UW>
 __global__ __launch_bounds__(256, 2) void score_max_i8_kernel(MaxArgs m)
@@ -139,9 +142,9 @@ __global__ __launch_bounds__(256, 2) void score_max_i8_kernel(MaxArgs m)
         const int64_t row = user_row(a, ur < a.n ? ur : a.n - 1, &id);
         sp[s] = a.sp[row];
         off_sp[s] = -12582912.f * sp[s];
-        err_sp[s] = sp[s] == sp[s] ? 1.6f * sp[s] : 0.f;       // (a user without a scale has no scores to bound)
+        err_sp[s] = sp[s] == sp[s] ? 1.6f * fabsf(sp[s]) : 0.f;        // (a user without a scale has no scores to bound)
         slack[s] = 0.f;
-        wide_user |= sp[s] > 0x1p50f;
+        wide_user |= fabsf(sp[s]) > 0x1p50f;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
             const int c = 32 * ks + 16 * h;
@@ -202,7 +205,7 @@ __global__ __launch_bounds__(256, 2) void score_max_i8_kernel(MaxArgs m)
         }
         float sqm = 0.f;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) sqm = fmaxf(sqm, sqv[e]);
+        for (int e = 0; e < 16; ++e) sqm = fmaxf(sqm, fabsf(sqv[e]));
         auto keep = [&](int s, float mx, float d) {
             slack[s] = fmaxf(slack[s], d);
             out[wave][s][2 * i + h][r] = mx + fmaf(fabsf(mx), 0x1p-21f, d);
@@ -284,7 +287,8 @@ __global__ __launch_bounds__(256, 2) void score_max_i8_kernel(MaxArgs m)
 // a workgroup's list of keys (scored by 256 threads; NT threads in all)
 // ------------------------------------------------------------------------------------------
 // LIST keys at most: room for k and for the 256 that one step may add.  512 up to k = 112 (a quarter of the registers and
-// half the LDS of 1024, which is what bounds the workgroups a CU holds: 110 -> see pick_i8_kernel), else 1024.
+// half the LDS of 1024, which is what bounds the workgroups a CU holds: pick_i8_kernel for 4096 users of 200k items 80 us
+// against 110), else 1024.
 static inline int list_for(int k) { return k <= 112 ? 512 : 1024; }
 template <int LIST>
 struct GroupList {
@@ -428,7 +432,9 @@ static constexpr int CAND = 2048;              // cells scored between two looks
 __device__ __forceinline__ int64_t cell_first(int64_t y) { return (y >> 1) * BLOCK + 4 * (y & 1); }
 __device__ __forceinline__ int64_t cell_item(int64_t y, int e) { return cell_first(y) + 8 * (e >> 2) + (e & 3); }
 
-// NT = 256 threads, or 1024 where there are few users and one workgroup's time is the call's; LPI: see RowDot
+// NT = 256 threads, or 1024 where there are few users and one workgroup's time is the call's; LPI: see RowDot.
+// Bound by latency, some twenty dependent steps a user: 4096 users of 200k items 78 us (five workgroups a CU; more of them
+// at fewer registers gain nothing), one user of 200k items 15 us, 33 of 2M items 27 us.
 template <int NT, int LPI, int LIST>
 __global__ __launch_bounds__(NT) void pick_i8_kernel(MaxArgs m)
 {
@@ -589,7 +595,8 @@ __global__ __launch_bounds__(NT) void pick_i8_kernel(MaxArgs m)
 }
 
 // ------------------------------------------------------------------------------------------
-// few items: a workgroup scores them all for one user, 16 per thread at most
+// few items: a workgroup scores them all for one user, 16 per thread at most (943 users of 1682 items, 20 columns: 18 us,
+// nearly all of it the dependent steps of one workgroup)
 // ------------------------------------------------------------------------------------------
 template <int LPI, int LIST>
 __global__ __launch_bounds__(256) void score_small_i8_kernel(ScoreI8Args a)
