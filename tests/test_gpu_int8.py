@@ -497,7 +497,7 @@ def test_product_tiles_into_a_pitched_slice(dev):
 
 @pytest.mark.parametrize("n,I,d,k,train", [
     (200, 6000, 100, 20, 10), (97, 4097, 128, 33, 5), (20, 8000, 128, 10, 3), (33, 9000, 200, 10, 5), (3, 120000, 64, 20, 30), (300, 120000, 20, 20, 30),
-    (40, 110000, 150, 5, 3), (260, 100001, 31, 113, 2)])
+    (40, 110000, 150, 5, 3), (260, 100001, 31, 113, 2), (300, 7000, 192, 20, 9), (30, 5001, 129, 20, 9)])
 def test_topk_sets_and_groups(dev, n, I, d, k, train):
     case = topk_case(n + I + d + k, n, I, d, train)
     check_topk(dev, case, np.arange(n)[::-1], k)
