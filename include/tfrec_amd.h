@@ -399,9 +399,11 @@ int tfrec_score_topk(tfrec_ctx *ctx, const float *d_P, const float *d_Q, const f
 /* tfrec_score_topk on tables that are kept in 8 bits (tfrec_quantize_rows_i8): scores as tfrec_matmul_i8 forms them,
  * score = ((float)sum * sp[user]) * sq[item] + b[item], each step rounded to float32; same order, masks and outputs.
  * d_Pq: the user table [U, ldp], indexed by user id (an id outside is clamped and raises the bad-index flag), or, with
- * p_compact = 1, the listed users' rows in list order (U >= n).  d_b [I] or null.  d <= 256, k <= 240, scales
- * non-negative.  A user or item whose scale is NaN has no scores (no entry / never listed).
- * Scratch comes from the context's workspace: call it once before capturing it into a HIP graph. */
+ * p_compact = 1, the listed users' rows in list order (U >= n; the listed ids are then used for the train CSR alone and
+ * have to be rows of it).  d_b [I] or null.  d <= 256, k <= 240.  A user or item whose scale is NaN has no scores (no
+ * entry / never listed).
+ * Scratch comes from the context's workspace: call it once before capturing it into a HIP graph; graphs captured from
+ * one context share that scratch and must not be replayed at the same time. */
 int tfrec_score_topk_i8(tfrec_ctx *ctx, const int8_t *d_Pq, int64_t ldp, const float *d_sp, int64_t U, int p_compact,
                         const int8_t *d_Qq, int64_t ldq, const float *d_sq, const float *d_b,
                         int64_t I, int d, int64_t item_lo, int64_t item_hi,

@@ -339,3 +339,22 @@ def test_clip_norm_of_sharded_and_adversarial_models_is_refused():
     ev = FoldOutEvaluator(data.train_matrix, data.test_matrix, top_k=5)
     with pytest.raises(ValueError, match="single-GPU"):
         make_model("BPR", data, ev, clip_norm=1.0, force_sharded=True)
+
+
+def test_a_list_is_not_made_under_capture(dev):
+    xs = [torch.ones(50000, device="cuda"), torch.ones(9000, device="cuda")]
+    norm = torch.zeros(1, device="cuda")
+    lst = dev.grad_list(xs)
+    dev.grad_norm(lst, norm=norm)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=dev._torch_stream):
+        with pytest.raises(ValueError):
+            dev.grad_list(xs)
+        dev.grad_norm(lst, norm=norm)
+    for v in (2.0, 3.0):
+        for x in xs:
+            x.fill_(v)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert abs(float(norm) - v * 59000 ** 0.5) <= 2.0 ** -23 * float(norm)

@@ -478,6 +478,24 @@ def test_product_tiles(dev, M, N, K, out):
     check_product(dev, A, sa * np.float32(0.02), B, sb, b, out)
 
 
+@pytest.mark.parametrize("M,N,K", [(130, 40001, 600), (300, 5003, 777), (20, 30001, 1030), (33, 70000, 520), (129, 41000, 640), (70, 9000, 4097), (128, 8193, 1281)])
+def test_product_tiles_of_few_rows(dev, M, N, K):
+    check_product(dev, *product_case(M + N + K, M, N, K, bias=M % 2 == 0))
+
+
+def test_product_of_rows_far_apart(dev):
+    """Rows 16 MiB apart: a tile's rows do not fit 32-bit offsets."""
+    M, N, K, ld = 66, 9000, 520, 1 << 24
+    A, sa, B, sb, b = product_case(7, M, N, K)
+    wide = torch.zeros(M, ld, dtype=torch.int8, device="cuda")
+    wide[:, :K] = torch.from_numpy(A).cuda()
+    from tfrec_amd.device import QuantRows
+    a, w, bias = QuantRows(wide, torch.from_numpy(sa).cuda(), K), quant_rows(B, sb, K), torch.from_numpy(b).cuda()
+    got, want = (dev.matmul_i8(x, w, bias=bias, out=torch.empty(M, N, device="cuda")) for x in (a, quant_rows(A, sa, K)))
+    dev.synchronize()
+    assert torch.equal(got, want)
+
+
 def test_product_tiles_into_a_pitched_slice(dev):
     """Every tile kernel into an output whose rows start off their 16 bytes; what lies around it stays."""
     for M, N, K in ((1000, 3301, 200), (500, 1101, 300), (2100, 4701, 512), (70, 131, 64)):
@@ -561,3 +579,23 @@ def test_captured_topk_with_scratch(dev, n, I):
         wide = quant_rows(big.cpu().numpy(), np.ones(len(big), np.float32), 64)
         dev.score_topk_i8(wide, wide, None, torch.arange(600 * (turn + 1), dtype=torch.int32, device="cuda"), 10)
         torch.cuda.synchronize()
+
+
+def test_freed_rows_are_refused_and_an_empty_train_matrix_masks_nothing(dev):
+    from tfrec_amd.device import QuantRows
+    rng = np.random.default_rng(4)
+    P, Q = rng.normal(0, 1, (3, 20)).astype(np.float32), rng.normal(0, 1, (50, 20)).astype(np.float32)
+    p, q = dev.quantize_rows(torch.from_numpy(P).cuda()), dev.quantize_rows(torch.from_numpy(Q).cuda())
+    users = torch.arange(3, dtype=torch.int32).cuda()
+    empty = torch.zeros(4, dtype=torch.int64).cuda(), torch.zeros(0, dtype=torch.int32).cuda()
+    want = dev.score_topk_i8(p, q, None, users, 5)
+    got = dev.score_topk_i8(p, q, None, users, 5, train=empty)
+    dev.synchronize()
+    assert np.array_equal(want[0].numpy(), got[0].numpy()) and np.array_equal(want[1].numpy(), got[1].numpy())
+    q.q.free()
+    with pytest.raises(ValueError):
+        dev.matmul_i8(p, q)
+    with pytest.raises(ValueError):
+        dev.score_topk_i8(p, q, None, users, 5)
+    with pytest.raises(ValueError):
+        QuantRows(torch.zeros(4, 64, dtype=torch.int8).cuda()[:, :32], torch.zeros(4).cuda(), 30)

@@ -442,6 +442,9 @@ extern "C" int tfrec_grads_create(tfrec_ctx *ctx, int n, const void *const *h_gr
     TF_TRY(check_grads(n, h_grads, h_counts, h_dtypes));
     TF_TRY(check_outputs(n, h_grads, h_out, h_counts, h_dtypes));
     TF_TRY(tfrec_ctx_enter(ctx));
+    hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+    TF_HIP(hipStreamIsCapturing(ctx->stream, &cap));
+    TF_REQUIRE(cap == hipStreamCaptureStatusNone, TFREC_EINVAL, "a list cannot be made while the stream is captured");
     int64_t chunks = 0;
     for (int i = 0; i < n; ++i) chunks += (h_counts[i] + GRAD_CHUNK - 1) / GRAD_CHUNK;
     tfrec_grads *g = new (std::nothrow) tfrec_grads();

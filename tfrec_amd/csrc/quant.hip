@@ -393,27 +393,29 @@ __global__ __launch_bounds__(256) void matmul_i8_kernel(MatmulArgs a)
 }
 
 // ---- large products: WM x WN waves, FM x FN blocks of 32 x 32 of C per wave ----------------------------------------------
-// Bound by the matrix cores.  256 x 256 of C per workgroup (2 x 4 waves of 4 x 2 blocks, two waves a SIMD), or 128 x 128
-// (2 x 2 waves of 2 x 2 blocks) where the larger tiles are too few for the chip.  A step takes 128 columns: 4 FM FN matrix
-// instructions a wave.  Rows go from memory straight into LDS (global_load_lds_dwordx4: one kilobyte, eight rows, per
-// instruction and wave), two buffers: the next step's loads are issued among this step's products.  The LDS image has no row padding; position
-// c of row r holds the row's chunk c ^ (r & 7), so that fragment reads spread over the banks (the swizzle is on the source
-// address).  Rows past the ends of A and B read the last row, columns past K are masked out of A's fragments in the last
-// step.  C goes out through LDS, so that stores cover whole 128-byte pieces of its rows.
-template <class T>
-using global_ptr = __attribute__((address_space(1))) T *;
-
-template <int WM, int WN, int FM, int FN>
+// 256 x 256 of C per workgroup (2 x 4 waves of 4 x 2 blocks, two waves a SIMD), bound by the matrix cores (8192 x 8192 x 8192
+// 482 us, 2.28 * 10^15 operations/s), or 128 x 128 (2 x 2 waves of 2 x 2 blocks) where the larger tiles are too few for the chip.
+// A step takes 128 columns: 4 FM FN matrix instructions a wave.  Rows go from memory straight into LDS
+// (global_load_lds_dwordx4: one kilobyte, eight rows, per instruction and wave), NB buffers: the loads of step s + NB - 1 are
+// issued among the products of step s.  The LDS image has no row padding; position c of row r holds the row's chunk c ^ (r & 7),
+// so that fragment reads spread over the banks (the swizzle is on the source address).  Rows past the ends of A and B read
+// the last row, columns past K are masked out of A's fragments in the last step.  C goes out through LDS, so that stores cover
+// whole 128-byte pieces of its rows.
+// With one workgroup a CU (NB = 4) a SIMD has one wave, and nothing hides its waits but itself: fragments are read two
+// products ahead, requests cost one vector instruction each (scalar base, 32-bit offsets).  A step is then 0.45 us, 0.7 without
+// (the products alone 0.21): 512 x 4096 x 8192 37 us.
+template <int WM, int WN, int FM, int FN, int NB>
 struct BigGeom {
     static constexpr int NW = WM * WN, SIDE = 32 * FM * WM, KB = 128, HALF = SIDE * KB, BUF = 2 * HALF;
-    static_assert(SIDE == 32 * FN * WN && SIDE / 8 == 4 * NW && FN == 2 && 2 * BUF / NW == 16384, "tiles are square, four loads a wave and side, 64 columns a wave");
-    static constexpr int LDS = 2 * BUF + SIDE * 4;     // two buffers, and A's scales
+    static_assert(SIDE == 32 * FN * WN && SIDE / 8 == 4 * NW && FN == 2 && 2 * BUF / NW == 16384 && NB >= 2 && NB <= 4, "tiles are square, four loads a wave and side, 64 columns a wave");
+    static constexpr int LDS = NB * BUF + SIDE * 4;    // the buffers, and A's scales
+    static_assert(LDS <= 160 << 10, "more than a CU's LDS");
 };
 
-template <class T, int WM, int WN, int FM, int FN>
+template <class T, int WM, int WN, int FM, int FN, int NB>
 __global__ __launch_bounds__((64 * WM * WN)) void matmul_i8_big_kernel(MatmulArgs a, int tiles_m, int tiles_n)
 {
-    using G = BigGeom<WM, WN, FM, FN>;
+    using G = BigGeom<WM, WN, FM, FN, NB>;
     constexpr int KB = G::KB, HALF = G::HALF, BUF = G::BUF, NW = G::NW, SIDE = G::SIDE;
     extern __shared__ __align__(16) char lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 31, h = lane >> 5;
@@ -426,62 +428,117 @@ __global__ __launch_bounds__((64 * WM * WN)) void matmul_i8_big_kernel(MatmulArg
     const int band_m = tiles_m - 4 * band < 4 ? tiles_m - 4 * band : 4;
     const int64_t m0 = (int64_t)(4 * band + in_band % band_m) * SIDE, n0 = (int64_t)(in_band / band_m) * SIDE;
 
-    // this wave's rows of a step: 8 * (NW i + wave) + lane / 8 of A and of B, i = 0..3
+    // this wave's rows of a step: 8 * (NW i + wave) + lane / 8 of A and of B, i = 0..3, as offsets from the tile's first rows
+    // (the launch code sees to it that they fit 32 bits); the step's columns are in the scalar base
     const int chunk = ((lane & 7) ^ (lane >> 3)) * 16;
-    global_ptr<const char> src[8];
+    uint32_t from[8];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const int64_t row = 8 * (NW * i + wave) + (lane >> 3);
-        src[i] = (global_ptr<const char>)(const char *)(a.A + (m0 + row < a.M ? m0 + row : a.M - 1) * a.lda);
-        src[4 + i] = (global_ptr<const char>)(const char *)(a.B + (n0 + row < a.N ? n0 + row : a.N - 1) * a.ldb);
+        const int row = 8 * (NW * i + wave) + (lane >> 3);
+        const int64_t last_a = a.M - 1 - m0, last_b = a.N - 1 - n0;
+        from[i] = (uint32_t)((row < last_a ? row : last_a) * a.lda) + chunk;
+        from[4 + i] = (uint32_t)((row < last_b ? row : last_b) * a.ldb) + chunk;
     }
-    float *scale_a = reinterpret_cast<float *>(lds + 2 * BUF);
+    const char *base_a = (const char *)a.A + m0 * a.lda, *base_b = (const char *)a.B + n0 * a.ldb;
+    float *scale_a = reinterpret_cast<float *>(lds + NB * BUF);
     if (tid < SIDE) scale_a[tid] = a.sa[m0 + tid < a.M ? m0 + tid : a.M - 1];
-    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
-    auto request = [&](int64_t k0, int buf, int i) {
-        const int64_t k = k0 + chunk;
-        const global_ptr<const char> from = src[i] + (k < a.K ? k : 0);
-        const uint32_t to = __builtin_amdgcn_readfirstlane(lds0 + (uint32_t)(buf * BUF + (i >> 2) * HALF + (NW * (i & 3) + wave) * 1024));
-        asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(to) : "memory", "m0");
+    const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds + wave * 1024);
+    const int steps = (int)((a.K + KB - 1) / KB);        // (K <= 131071)
+    // load i of step s into buffer buf; lanes whose chunk of the last step begins past K read its first
+    auto request = [&](int s, int buf, int i) {
+        const uint32_t back = s + 1 == steps && s * KB + chunk >= (int)a.K ? chunk : 0;
+        const char *base = (i < 4 ? base_a : base_b) + s * KB;
+        const uint32_t to = lds0 + buf * BUF + (i >> 2) * HALF + NW * (i & 3) * 1024;
+        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(from[i] - back), "s"(base), "s"(to) : "memory", "m0");
     };
     const int wm = wave / WN * (32 * FM), wn = wave % WN * (32 * FN);
     int off[KB / 32];
 #pragma unroll
     for (int ks = 0; ks < KB / 32; ++ks) off[ks] = r * KB + (((2 * ks + h) ^ (r & 7)) * 16);
     i32x16 acc[FM][FN] = {};
-    const int64_t steps = (a.K + KB - 1) / KB;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) request(0, 0, i);
-    for (int64_t s = 0; s < steps; ++s) {
-        const int buf = (int)(s & 1);
-        const bool last = s + 1 == steps;
-        // this wave's loads of the step have landed, and after the barrier everyone's; everyone is also done with the other buffer
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    for (int q = 0; q < NB - 1; ++q)
+        if (q < steps)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) request(q, q, i);
+    // Step s's rows are here: this wave's loads of it have landed (of up to NB - 2 later steps 8 each may be under way; loads
+    // return in order, and there are no others), after the barrier everyone's; and everyone's earlier fragment reads are done.
+    auto landed = [&](int s) {
+        if (NB > 3 && s + 2 < steps) asm volatile("s_waitcnt vmcnt(16) lgkmcnt(0)" ::: "memory");
+        else if (NB > 2 && s + 1 < steps) asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)" ::: "memory");
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
+    };
+    constexpr int KS = KB / 32, SLOTS = NB == 2 ? 2 : KS;
+    i32x4 fa[SLOTS][FM], fb[SLOTS][FN];
+    auto fragments = [&](int buf, int ks) {
         const char *A = lds + buf * BUF + wm * KB, *B = lds + buf * BUF + HALF + wn * KB;
-        i32x4 fa[2][FM], fb[2][FN];
-        auto fragments = [&](int ks, int to) {
+        const int to = ks % SLOTS;
 #pragma unroll
-            for (int i = 0; i < FM; ++i) fa[to][i] = *reinterpret_cast<const i32x4 *>(A + off[ks] + 32 * i * KB);
+        for (int i = 0; i < FM; ++i) fa[to][i] = *reinterpret_cast<const i32x4 *>(A + off[ks] + 32 * i * KB);
 #pragma unroll
-            for (int j = 0; j < FN; ++j) fb[to][j] = *reinterpret_cast<const i32x4 *>(B + off[ks] + 32 * j * KB);
-            if (last)
+        for (int j = 0; j < FN; ++j) fb[to][j] = *reinterpret_cast<const i32x4 *>(B + off[ks] + 32 * j * KB);
+    };
+    // columns from K on (in the last step) count as zeros
+    auto cut = [&](int ks) {
 #pragma unroll
-                for (int i = 0; i < FM; ++i) fa[to][i] = __builtin_bit_cast(i32x4, keep_below(__builtin_bit_cast(uint4, fa[to][i]), s * KB + 32 * ks + 16 * h, a.K));
-        };
-        fragments(0, 0);
+        for (int i = 0; i < FM; ++i)
+            fa[ks % SLOTS][i] = __builtin_bit_cast(i32x4, keep_below(__builtin_bit_cast(uint4, fa[ks % SLOTS][i]), (steps - 1) * KB + 32 * ks + 16 * h, a.K));
+    };
+    auto products = [&](int ks) {
 #pragma unroll
-        for (int ks = 0; ks < KB / 32; ++ks) {
-            if (ks + 1 < KB / 32) fragments(ks + 1, (ks + 1) & 1);
-            if (!last) {
-                request((s + 1) * KB, buf ^ 1, 2 * ks);
-                request((s + 1) * KB, buf ^ 1, 2 * ks + 1);
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa[ks % SLOTS][i], fb[ks % SLOTS][j], acc[i][j], 0, 0, 0);
+    };
+    if constexpr (NB == 2) {
+        for (int s = 0; s < steps; ++s) {
+            const int buf = s & 1;
+            const bool last = s + 1 == steps;
+            landed(s);
+            fragments(buf, 0);
+            if (last) cut(0);
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                if (ks + 1 < KS) {
+                    fragments(buf, ks + 1);
+                    if (last) cut(ks + 1);
+                }
+                if (!last) {
+                    request(s + 1, buf ^ 1, 2 * ks);
+                    request(s + 1, buf ^ 1, 2 * ks + 1);
+                }
+                products(ks);
             }
+        }
+    } else {
+        // one wave a SIMD: fragments are read two products ahead, past the barrier between two steps
+        landed(0);
+        fragments(0, 0);
+        fragments(0, 1);
+        int buf = 0;
+        for (int s = 0; s + 1 < steps; ++s) {
+            const int before = buf == 0 ? NB - 1 : buf - 1, next = buf + 1 == NB ? 0 : buf + 1;      // the buffers of steps s - 1 and s + 1
 #pragma unroll
-            for (int i = 0; i < FM; ++i)
+            for (int ks = 0; ks < KS; ++ks) {
+                if (ks + 2 == KS) landed(s + 1);
+                fragments(ks + 2 < KS ? buf : next, (ks + 2) % KS);
+                if (ks < 2 && s + NB - 1 < steps)
 #pragma unroll
-                for (int j = 0; j < FN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa[ks & 1][i], fb[ks & 1][j], acc[i][j], 0, 0, 0);
+                    for (int i = 4 * ks; i < 4 * ks + 4; ++i) request(s + NB - 1, before, i);
+                __builtin_amdgcn_sched_barrier(0);
+                products(ks);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            buf = next;
+        }
+        fragments(buf, 2);
+        fragments(buf, 3);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            cut(ks);
+            products(ks);
         }
     }
     __syncthreads();
@@ -522,34 +579,41 @@ __global__ __launch_bounds__((64 * WM * WN)) void matmul_i8_big_kernel(MatmulArg
     }
 }
 
-template <class T, int WM, int WN, int FM, int FN>
+template <class T, int WM, int WN, int FM, int FN, int NB>
 static int launch_big(tfrec_ctx *ctx, const MatmulArgs &a)
 {
-    using G = BigGeom<WM, WN, FM, FN>;
+    using G = BigGeom<WM, WN, FM, FN, NB>;
     const int64_t tm = (a.M + G::SIDE - 1) / G::SIDE, tn = (a.N + G::SIDE - 1) / G::SIDE, tiles = tm * tn;
     TF_REQUIRE(tiles < (1ll << 28), TFREC_EUNSUP, "the product is too large for one launch");
     static std::atomic<uint64_t> done{0};
-    TF_TRY(tfrec_raise_lds_limit(ctx, reinterpret_cast<const void *>(&matmul_i8_big_kernel<T, WM, WN, FM, FN>), G::LDS, done));
-    matmul_i8_big_kernel<T, WM, WN, FM, FN><<<(unsigned)((tiles + 7) / 8 * 8), 64 * G::NW, G::LDS, ctx->stream>>>(a, (int)tm, (int)tn);
+    TF_TRY(tfrec_raise_lds_limit(ctx, reinterpret_cast<const void *>(&matmul_i8_big_kernel<T, WM, WN, FM, FN, NB>), G::LDS, done));
+    matmul_i8_big_kernel<T, WM, WN, FM, FN, NB><<<(unsigned)((tiles + 7) / 8 * 8), 64 * G::NW, G::LDS, ctx->stream>>>(a, (int)tm, (int)tn);
     TF_HIP(hipGetLastError());
     return TFREC_OK;
 }
 
 // Which kernel (us, measured on both sides of each rule):
 //   256 x 256 tiles where they fill the chip and a row is long enough to repay 128 KB of LDS, one workgroup a CU
-//     (4096 x 8192 x 8192: 264; 128 x 128 tiles 330 at the same rows);
-//   128 x 128 tiles of the same kernel for 64 rows of A and more, once there are 32 of them: 512 x 4096 x 4096 27 against 69
-//     for 16 rows of B at a time, 256 x 4096 x 4096 22 / 37, 128 x 4096 x 4096 even, 333 x 555 x 7777 (15 tiles) 39 / 31;
-//   rows below 256 columns are bound by the stores of C, which the kernel with 33 KB of LDS and several workgroups a CU
-//     serves best: 2048 x 200000 x 64 in float32 310 (5.3 TB/s; a fill of C alone 240) against 454;
+//     (4096 x 8192 x 8192: 254; 128 x 128 tiles 284 to 370);
+//   128 x 128 tiles where the time that reading B for 16 of its rows at a time takes (what a sweep over M, N and K measured:
+//     more with every row of A) exceeds that of the tiles, a chain of K / 128 steps: 16 x 65536 x 4096 47 / 70,
+//     512 x 4096 x 4096 22 / 69, 77 x 5003 x 1210 11 / 8.9, 128 x 4096 x 4096 20 / 21, 1 x 8192 x 8192 34 / 15.  Up to one tile a CU with
+//     four buffers (512 x 8192 x 4096: 26, with two 32), beyond with two and two workgroups a CU (1024 x 8192 x 4096: 40, 51);
+//   short rows (512 columns and a float32 output, 256 and 16 bits) are bound by the stores of C, which the kernel with 33 KB of
+//     LDS and several workgroups a CU serves best: 2048 x 200000 x 64 in float32 300 (5.5 TB/s; a fill of C alone 240) against
+//     454, 2048 x 50000 x 256 in float32 113 / 151, in bfloat16 even, x 512 even / in bfloat16 128 / 100;
 //   16 rows of B at a time for everything else: small products get workgroups enough, few rows of A are bound by reading B.
 template <class T>
 static int launch_matmul(tfrec_ctx *ctx, const MatmulArgs &a)
 {
     const int64_t big = ((a.M + 255) / 256) * ((a.N + 255) / 256), mid = ((a.M + 127) / 128) * ((a.N + 127) / 128);
-    if (a.K >= 512 && big >= 160) return launch_big<T, 2, 4, 4, 2>(ctx, a);
-    if (a.M > 64 && mid >= 32 && a.K >= 256) return launch_big<T, 2, 2, 2, 2>(ctx, a);
-    if (a.M > 64 && mid >= 192) {
+    const bool near = a.lda < (1 << 24) && a.ldb < (1 << 24);        // a tile's rows are within 4 GB of its first
+    const double rows_us = (double)a.N * (double)a.K * (1.6e-7 + 6.2e-9 * (double)a.M);
+    const double tiles_us = (2.2 + 3.65e-3 * (double)a.K) * (mid > 256 ? (double)mid / 230. : 1.);
+    const bool stores = a.M > 64 && mid >= 192 && a.K <= 128 * (int64_t)sizeof(T);
+    if (near && !stores && a.M > 128 && a.K >= 512 && big >= 160) return launch_big<T, 2, 4, 4, 2, 2>(ctx, a);
+    if (near && !stores && a.K >= 256 && rows_us > tiles_us) return mid <= 256 ? launch_big<T, 2, 2, 2, 2, 4>(ctx, a) : launch_big<T, 2, 2, 2, 2, 2>(ctx, a);
+    if (stores || (a.M > 64 && mid >= 192)) {
         TF_REQUIRE(mid < (1ll << 31), TFREC_EUNSUP, "the product is too large for one launch");
         matmul_i8_kernel<T><<<(unsigned)mid, 256, 0, ctx->stream>>>(a);
     } else {

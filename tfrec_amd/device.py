@@ -131,8 +131,7 @@ class QuantRows:
         self.q, self.scale, self.d = q, scale, d
         self.shape = (shape[0], d)
         self.ld = shape[1]
-        # (the description of a matrix that stays where it is: looked up once, not at every call)
-        self.at = _ptr(q), _ptr(scale)
+        _ptr(q), _ptr(scale)            # (buffers, and contiguous)
         where = {_gpu_of(q), _gpu_of(scale)}
         if len(where) != 1:
             raise ValueError("q and scale are on different devices")
@@ -142,7 +141,7 @@ class QuantRows:
         """(address of q, address of scale), refused where they are not on ``dev``'s GPU."""
         if self.gpu != dev.device:
             raise ValueError("the 8-bit matrix is on %s, the context on GPU %d" % ("the host" if self.gpu is None else "GPU %d" % self.gpu, dev.device))
-        return self.at
+        return _ptr(self.q), _ptr(self.scale)
 
     def __len__(self):
         return self.shape[0]
@@ -674,6 +673,8 @@ class Device:
         out_scores = out_scores if out_scores is not None else self.empty((n, k), np.float32)
         if _shape(out_ids) != (n, k) or _dtype_name(out_ids) != "int32" or _shape(out_scores) != (n, k) or _dtype_name(out_scores) != "float32":
             raise ValueError("outputs must be int32 and float32 [%d, %d]" % (n, k))
+        if train is not None and _numel(train[1]) == 0:
+            train = None                # (no user has train items; such an array has no address)
         tp, ti = (train if train is not None else (None, None))
         if train is not None and (_dtype_name(tp) != "int64" or _dtype_name(ti) != "int32" or (not compact and _shape(tp)[0] <= U)):
             raise ValueError("train needs int64 row starts (one more than users) and int32 items")
