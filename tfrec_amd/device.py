@@ -214,8 +214,11 @@ def _gpu_of(x):
     """Ordinal of the GPU a buffer lives on; None for host memory."""
     if isinstance(x, (DevArray, DevView)):
         return x.dev.device
-    where = getattr(x, "device", None)
-    return where.index if where is not None and where.type == "cuda" else None
+    where = getattr(x, "get_device", None)          # (torch: -1 for host memory)
+    if where is None:
+        return None
+    where = where()
+    return where if where >= 0 else None
 
 
 def _dt(x):
@@ -235,32 +238,38 @@ def _numel(x):
 
 def _ptr_on(dev, x):
     """``_ptr`` of a buffer that has to live on ``dev``'s GPU."""
-    if x is not None and not isinstance(x, int) and _gpu_of(x) != dev.device:
+    if x is None:
+        return None
+    if _gpu_of(x) != dev.device and not isinstance(x, int):
         raise ValueError("the buffer is on %s, the context on GPU %d" % (getattr(x, "device", "another GPU"), dev.device))
     return _ptr(x)
 
 
 def _rows2d(dev, x, name):
     """(pointer, row pitch in elements) of a matrix whose rows are contiguous (a torch tensor may have a row pitch)."""
-    if len(_shape(x)) != 2:
+    shape = x.shape
+    if len(shape) != 2:
         raise ValueError("%s must be a matrix" % name)
     if hasattr(x, "data_ptr") and not isinstance(x, (DevArray, DevView)):
-        if x.shape[1] > 1 and x.stride(1) != 1:
+        n, d = shape
+        row, col = x.stride()
+        if d > 1 and col != 1:
             raise ValueError("%s: the values of a row must be contiguous" % name)
-        if x.device.type != "cuda" or x.device.index != dev.device:
+        if _gpu_of(x) != dev.device:
             raise ValueError("%s is on %s, the context on GPU %d" % (name, x.device, dev.device))
-        pitch = x.stride(0) if x.shape[0] > 1 else max(int(x.shape[1]), 1)
-        if pitch < x.shape[1]:
+        if n <= 1:
+            row = max(d, 1)
+        if row < d:
             raise ValueError("%s: rows overlap" % name)
-        return x.data_ptr(), pitch
-    return _ptr_on(dev, x), _shape(x)[1]
+        return x.data_ptr(), row
+    return _ptr_on(dev, x), shape[1]
 
 
 def _vector(dev, x, n, dtype, name):
     """Pointer of a contiguous device vector of ``n`` values of ``dtype`` (None passes)."""
     if x is None:
         return None
-    if _shape(x) != (n,) or _dtype_name(x) != dtype:
+    if x.shape != (n,) or _dtype_name(x) != dtype:
         raise ValueError("%s must be %s [%d]" % (name, dtype, n))
     return _ptr_on(dev, x)
 
@@ -271,12 +280,13 @@ def _ptr(x):
         return None
     if isinstance(x, (DevArray, DevView)):
         return x.ptr
-    if isinstance(x, int):
-        return x
-    if hasattr(x, "data_ptr"):
+    at = getattr(x, "data_ptr", None)
+    if at is not None:
         if not x.is_contiguous():
             raise ValueError("tensor must be contiguous")
-        return x.data_ptr()
+        return at()
+    if isinstance(x, int):
+        return x
     raise TypeError("not a device buffer: %r" % type(x))
 
 
@@ -586,7 +596,7 @@ class Device:
         if K != KB:
             raise ValueError("A has %d columns, B %d" % (K, KB))
         out = out if out is not None else self.empty((M, N), np.float32)
-        if _shape(out) != (M, N):
+        if out.shape != (M, N):
             raise ValueError("out must be [%d, %d]" % (M, N))
         cp, ldc = _rows2d(self, out, "out")
         aq, sa = A.on(self)
@@ -671,7 +681,7 @@ class Device:
         lo, hi = item_range if item_range is not None else (0, I)
         out_ids = out_ids if out_ids is not None else self.empty((n, k), np.int32)
         out_scores = out_scores if out_scores is not None else self.empty((n, k), np.float32)
-        if _shape(out_ids) != (n, k) or _dtype_name(out_ids) != "int32" or _shape(out_scores) != (n, k) or _dtype_name(out_scores) != "float32":
+        if out_ids.shape != (n, k) or _dtype_name(out_ids) != "int32" or out_scores.shape != (n, k) or _dtype_name(out_scores) != "float32":
             raise ValueError("outputs must be int32 and float32 [%d, %d]" % (n, k))
         if train is not None and _numel(train[1]) == 0:
             train = None                # (no user has train items; such an array has no address)
