@@ -288,7 +288,7 @@ __global__ __launch_bounds__(256, 2) void score_max_i8_kernel(MaxArgs m)
 // ------------------------------------------------------------------------------------------
 // LIST keys at most: room for k and for the 256 that one step may add.  512 up to k = 112 (a quarter of the registers and
 // half the LDS of 1024, which is what bounds the workgroups a CU holds: pick_i8_kernel for 4096 users of 200k items 80 us
-// against 110), else 1024.
+// against 110 when it was chosen), else 1024.
 static inline int list_for(int k) { return k <= 112 ? 512 : 1024; }
 template <int LIST>
 struct GroupList {
@@ -381,6 +381,28 @@ __device__ __forceinline__ void group_append(List &g, bool pass, uint64_t key)
     if (pass) g.list[base + __popcll(m & ((1ull << lane) - 1))] = key;
 }
 
+// The same for N keys a lane (key(i) is 0 for none) with one atomic a wave, and no look at the room: keys behind the list's end
+// are dropped, the count tells (the caller then goes over them again, checked).
+template <int N, int LIST, class Key>
+__device__ __forceinline__ void group_append_many(GroupList<LIST> &g, Key &&key)
+{
+    const int lane = threadIdx.x & 63;
+    int mine = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) mine += key(i) != 0;
+    const int incl = wave_prefix_sum(mine), total = __builtin_amdgcn_readlane(incl, 63);
+    if (!total) return;
+    int base = 0;
+    if (lane == 0) base = atomicAdd(&g.count, total);
+    int at = __builtin_amdgcn_readfirstlane(base) + incl - mine;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const uint64_t k = key(i);
+        if (k != 0 && at < LIST) g.list[at] = k;
+        at += k != 0;
+    }
+}
+
 // called by all threads after a step that appended at most 256 keys: cuts the list back to its k best once the next step might
 // not fit
 template <int LIST>
@@ -433,8 +455,9 @@ __device__ __forceinline__ int64_t cell_first(int64_t y) { return (y >> 1) * BLO
 __device__ __forceinline__ int64_t cell_item(int64_t y, int e) { return cell_first(y) + 8 * (e >> 2) + (e & 3); }
 
 // NT = 256 threads, or 1024 where there are few users and one workgroup's time is the call's; LPI: see RowDot.
-// Bound by latency, some twenty dependent steps a user: 4096 users of 200k items 78 us (five workgroups a CU; more of them
-// at fewer registers gain nothing), one user of 200k items 15 us, 33 of 2M items 27 us.
+// Bound by latency, some twenty dependent steps a user: 4096 users of 200k items 68 to 75 us (five workgroups a CU; more of
+// them at fewer registers gain nothing; with a look at the list's room every 256 items 80), one user of 200k items 15 us, 33
+// of 2M items 25 us.
 template <int NT, int LPI, int LIST>
 __global__ __launch_bounds__(NT) void pick_i8_kernel(MaxArgs m)
 {
@@ -538,52 +561,69 @@ __global__ __launch_bounds__(NT) void pick_i8_kernel(MaxArgs m)
                 const uint32_t u = units[v0 + i / sub], y = u * sub + i % sub;
                 if (make_key(bound[y], (int32_t)(id0 + cell_first(y))) > kth) cand[atomicAdd(&n_cand, 1)] = y;
             }
+            const int held = g.count;
             __syncthreads();
             const int c = n_cand;
-            for (int c0 = 0; c0 < c * CELL; c0 += 256 * ROUNDS) {
-                int acc[ROUNDS];
-                int64_t own[ROUNDS];
-                typename RowDot<LPI>::Scale sc[ROUNDS];
-                if (tid < 256) {
-                    uint4 q[ROUNDS][LPI];
-#pragma unroll
-                    for (int o = 0; o < ROUNDS; ++o) {
-                        const int i = c0 + 256 * o + RowDot<LPI>::owned();
-                        own[o] = i < c * CELL ? cell_item(cand[i / CELL], i % CELL) : a.n_items;
-                        sc[o] = dot.scale(a, own[o] < a.n_items ? own[o] : 0);
-                    }
-#pragma unroll
-                    for (int o = 0; o < ROUNDS; ++o)
-#pragma unroll
-                        for (int j = 0; j < LPI; ++j) {
-                            const int i = c0 + 256 * o + j * (256 / LPI) + tid / LPI;
-                            int64_t it = i < c * CELL ? cell_item(cand[i / CELL], i % CELL) : 0;
-                            it = it < a.n_items ? it : 0;
-                            q[o][j] = dot.load(a, it);
-                        }
-#pragma unroll
-                    for (int o = 0; o < ROUNDS; ++o)
-#pragma unroll
-                        for (int j = 0; j < LPI; ++j) {
-                            const int s = dot.dot(q[o][j]);
-                            if (tid % LPI == j) acc[o] = s;
-                        }
-                }
-#pragma unroll
-                for (int o = 0; o < ROUNDS; ++o) {
-                    if (o > 0 && c0 + 256 * o >= c * CELL) break;
+            // once without a look at the list's room (the cut lets little more than k items pass), and once more, checked
+            // every 256 items, where it did not do
+#pragma unroll 1
+            for (int turn = 0;; ++turn) {
+                for (int c0 = 0; c0 < c * CELL; c0 += 256 * ROUNDS) {
+                    int acc[ROUNDS];
+                    int64_t own[ROUNDS];
+                    typename RowDot<LPI>::Scale sc[ROUNDS];
                     if (tid < 256) {
-                        bool pass = false;
-                        uint64_t k64 = 0;
-                        if (own[o] < a.n_items) {
-                            const float v = dot.score(acc[o], sc[o]);
-                            k64 = make_key(v, (int32_t)(id0 + own[o]));
-                            pass = v > -INFINITY && k64 > g.kth;
+                        uint4 q[ROUNDS][LPI];
+#pragma unroll
+                        for (int o = 0; o < ROUNDS; ++o) {
+                            const int i = c0 + 256 * o + RowDot<LPI>::owned();
+                            own[o] = i < c * CELL ? cell_item(cand[i / CELL], i % CELL) : a.n_items;
+                            sc[o] = dot.scale(a, own[o] < a.n_items ? own[o] : 0);
                         }
-                        group_append(g, pass, k64);
+#pragma unroll
+                        for (int o = 0; o < ROUNDS; ++o)
+#pragma unroll
+                            for (int j = 0; j < LPI; ++j) {
+                                const int i = c0 + 256 * o + j * (256 / LPI) + tid / LPI;
+                                int64_t it = i < c * CELL ? cell_item(cand[i / CELL], i % CELL) : 0;
+                                it = it < a.n_items ? it : 0;
+                                q[o][j] = dot.load(a, it);
+                            }
+#pragma unroll
+                        for (int o = 0; o < ROUNDS; ++o)
+#pragma unroll
+                            for (int j = 0; j < LPI; ++j) {
+                                const int s = dot.dot(q[o][j]);
+                                if (tid % LPI == j) acc[o] = s;
+                            }
                     }
-                    group_check(g, a.k, a.train_indices, mlo, mhi);
+                    uint64_t k64[ROUNDS];
+                    if (tid < 256)
+#pragma unroll
+                        for (int o = 0; o < ROUNDS; ++o) {
+                            const float v = dot.score(acc[o], sc[o]);
+                            k64[o] = own[o] < a.n_items && v > -INFINITY ? make_key(v, (int32_t)(id0 + own[o])) : 0;
+                        }
+                    if (turn == 0) {
+                        const uint64_t least = g.kth;
+                        if (tid < 256) group_append_many<ROUNDS>(g, [&](int o) { return k64[o] > least ? k64[o] : 0; });
+                    } else {
+#pragma unroll 1
+                        for (int o = 0; o < ROUNDS && c0 + 256 * o < c * CELL; ++o) {
+                            uint64_t mine = k64[0];
+#pragma unroll
+                            for (int i = 1; i < ROUNDS; ++i) mine = i == o ? k64[i] : mine;
+                            if (tid < 256) group_append(g, mine > g.kth, mine);
+                            group_check(g, a.k, a.train_indices, mlo, mhi);
+                        }
+                    }
                 }
+                if (turn) break;
+                __syncthreads();
+                if (g.count <= LIST) break;
+                __syncthreads();
+                if (tid == 0) g.count = held;
+                group_check(g, a.k, a.train_indices, mlo, mhi);
             }
             if (tid == 0) n_cand = 0;
             __syncthreads();
@@ -595,7 +635,7 @@ __global__ __launch_bounds__(NT) void pick_i8_kernel(MaxArgs m)
 }
 
 // ------------------------------------------------------------------------------------------
-// few items: a workgroup scores them all for one user, 16 per thread at most (943 users of 1682 items, 20 columns: 18 us,
+// few items: a workgroup scores them all for one user, 16 per thread at most (943 users of 1682 items, 20 columns: 16.6 us,
 // nearly all of it the dependent steps of one workgroup)
 // ------------------------------------------------------------------------------------------
 template <int LPI, int LIST>
@@ -658,12 +698,23 @@ __global__ __launch_bounds__(256) void score_small_i8_kernel(ScoreI8Args a)
     const uint32_t cut = rank_bound<256, V>(key, KEY_NONE, a.k, g);
     if (tid == 0) g.kth = cut ? ((uint64_t)cut << 32) - 1 : ((uint64_t)KEY_NONE << 32 | 0xffffffffu);
     __syncthreads();
+    // (as in pick_i8_kernel: all keys at once where they fit the list, else 256 at a time)
+    auto k64 = [&](int v) { return ((uint64_t)key[v] << 32) | (uint32_t)~(uint32_t)(id0 + 256 * v + own); };
+    const uint64_t least = g.kth;
+    group_append_many<V>(g, [&](int v) { return key[v] > KEY_NONE && k64(v) > least ? k64(v) : 0; });
+    __syncthreads();
+    if (g.count > LIST) {
+        __syncthreads();
+        if (tid == 0) g.count = 0;
+        __syncthreads();
+#pragma unroll 1
+        for (int v = 0; 256 * v < n_items; ++v) {
+            uint64_t mine = k64(0);
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-        if (256 * v >= n_items) continue;
-        const uint64_t k64 = ((uint64_t)key[v] << 32) | (uint32_t)~(uint32_t)(id0 + 256 * v + own);
-        group_append(g, key[v] > KEY_NONE && k64 > g.kth, k64);
-        group_check(g, a.k, nullptr, 0, 0);
+            for (int i = 1; i < V; ++i) mine = i == v ? k64(i) : mine;
+            group_append(g, (uint32_t)(mine >> 32) > KEY_NONE && mine > g.kth, mine);
+            group_check(g, a.k, nullptr, 0, 0);
+        }
     }
     group_finish(g, a, r, nullptr, 0, 0);
 }
