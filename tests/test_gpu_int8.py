@@ -599,3 +599,29 @@ def test_freed_rows_are_refused_and_an_empty_train_matrix_masks_nothing(dev):
         dev.score_topk_i8(p, q, None, users, 5)
     with pytest.raises(ValueError):
         QuantRows(torch.zeros(4, 64, dtype=torch.int8).cuda()[:, :32], torch.zeros(4).cuda(), 30)
+
+
+def test_two_contexts_on_their_own_streams(dev):
+    """Calls of two contexts that overlap: each has scratch of its own."""
+    from tfrec_amd.device import Device
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    devs = [Device(0, s.cuda_stream) for s in streams]
+    cases = [topk_case(50 + i, 300, 20000, 40, 8) for i in range(2)]
+    held, want = [], []
+    for Pq, sp, Qq, sq, b, masks in cases:
+        held.append((quant_rows(Pq, sp, 40), quant_rows(Qq, sq, 40), torch.from_numpy(b).cuda(), torch.arange(300, dtype=torch.int32).cuda(), csr(masks)))
+        want.append(expected_topk(scores_f32(Pq, sp, Qq, sq, b), 20, masks))
+    torch.cuda.synchronize()
+    got = []
+    for turn in range(6):
+        for i, d in enumerate(devs):
+            p, q, b, users, train = held[i]
+            got.append((i, d.score_topk_i8(p, q, b, users, 20, train=train), d.matmul_i8(p, q, bias=b)))
+    for d in devs:
+        d.synchronize()
+    for i, (ids, sc), C in got:
+        assert np.array_equal(ids.numpy(), want[i][0]) and np.array_equal(sc.numpy(), want[i][1])
+        assert np.array_equal(C.numpy()[:2], scores_f32(*cases[i][:5])[:2])
+    del got, C, ids, sc
+    for d in devs:
+        d.close()

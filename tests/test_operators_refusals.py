@@ -239,3 +239,20 @@ def test_list_refusals(lib):
     refused(lib, lib.tfrec_grads_norm(None, None, A16), _lib.EINVAL, "null list")
     refused(lib, lib.tfrec_grads_clip(None, None, 1.0, A16), _lib.EINVAL, "null list")
     assert lib.tfrec_grads_destroy(None, None) == _lib.OK
+
+
+def test_gradient_tables_that_overlap_are_refused(lib):
+    U, I, d = 10, 20, 8
+    P, Q, b, gP, gQ, gb = (A16 + k * 4096 for k in range(6))
+
+    def call(**kw):
+        t = dict(P=P, Q=Q, b=b, gP=gP, gQ=gQ, gb=gb)
+        t.update(kw)
+        return lib.tfrec_bpr_grads(None, t["P"], t["Q"], t["b"], U, I, d, A16, A16, A16, 5, 0.1, t["gP"], t["gQ"], t["gb"], None)
+    refused(lib, call(), _lib.EINVAL, "null context")
+    refused(lib, call(gP=None), _lib.EINVAL, "null gradient")
+    for kw in (dict(gQ=gP), dict(gb=gQ + I * d * 4 - 4), dict(gP=gQ - U * d * 4 + 4), dict(gb=gP)):
+        refused(lib, call(**kw), _lib.EINVAL, "two gradient tables overlap")
+    for kw in (dict(gP=P), dict(gQ=Q + 4), dict(gb=b), dict(gP=Q), dict(gb=P + U * d * 4 - 4)):
+        refused(lib, call(**kw), _lib.EINVAL, "overlaps the parameters")
+    refused(lib, call(gQ=gP + U * d * 4, gb=gP + (U + I) * d * 4), _lib.EINVAL, "null context")

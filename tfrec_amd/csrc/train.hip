@@ -1299,7 +1299,14 @@ extern "C" int tfrec_bpr_grads(tfrec_ctx *ctx, const float *d_P, const float *d_
                                float *d_gQ, float *d_gb, double *d_loss)
 {
     TF_REQUIRE(d_gP && d_gQ && d_gb, TFREC_EINVAL, "null gradient table");
-    TF_REQUIRE(d_gP != d_P && d_gQ != d_Q && d_gb != d_b, TFREC_EINVAL, "gradients cannot replace the parameters");
+    if (U > 0 && I > 0 && d > 0) {
+        const float *at[6] = {d_gP, d_gQ, d_gb, d_P, d_Q, d_b};
+        const int64_t len[6] = {U * d, I * d, I, U * d, I * d, I};
+        for (int i = 0; i < 3; ++i)
+            for (int j = i + 1; j < 6; ++j)
+                TF_REQUIRE(!at[j] || (uintptr_t)(at[i] + len[i]) <= (uintptr_t)at[j] || (uintptr_t)(at[j] + len[j]) <= (uintptr_t)at[i], TFREC_EINVAL,
+                           j < 3 ? "two gradient tables overlap" : "a gradient table overlaps the parameters");
+    }
     TF_TRY(tfrec_ctx_enter(ctx));
     TF_TRY(check_step_args(d_P, d_Q, d_b, U, I, d, d_users, d_pos, d_neg, B));
     zero_tables_kernel<<<2048, 256, 0, ctx->stream>>>(d_gP, U * d, d_gQ, I * d, d_gb, I);
