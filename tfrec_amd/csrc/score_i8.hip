@@ -284,7 +284,7 @@ __global__ __launch_bounds__(256, 2) void score_max_i8_kernel(MaxArgs m)
 }
 
 // ------------------------------------------------------------------------------------------
-// a workgroup's list of keys (scored by 256 threads; NT threads in all)
+// a workgroup's list of keys
 // ------------------------------------------------------------------------------------------
 // LIST keys at most: room for k and for the 256 that one step may add.  512 up to k = 112 (a quarter of the registers and
 // half the LDS of 1024, which is what bounds the workgroups a CU holds: pick_i8_kernel for 4096 users of 200k items 80 us
@@ -540,7 +540,9 @@ __global__ __launch_bounds__(NT) void pick_i8_kernel(MaxArgs m)
     if (tid == 0) g.kth = T > -INFINITY ? ((uint64_t)f32_orderable(T) << 32) - 1 : ((uint64_t)KEY_NONE << 32 | 0xffffffffu);
     __syncthreads();
 
-    constexpr int ROUNDS = LPI <= 2 ? 4 : (LPI <= 8 ? 2 : 1);          // rounds of 256 items whose rows are requested together
+    // 256 threads (a team) score 256 items in a round; the rows of ROUNDS rounds are requested together
+    constexpr int TEAMS = NT / 256, ROUNDS = TEAMS > 1 ? (LPI <= 2 ? 2 : 1) : (LPI <= 2 ? 4 : (LPI <= 8 ? 2 : 1)), STEP = 256 * TEAMS * ROUNDS;
+    const int team = tid >> 8, lane_row = (tid & 255) / LPI;
     const int sub = by_group ? 16 : 1;                                  // cells of a unit
     const uint32_t per = (count + SLICES - 1) / SLICES, total = dot.sp == dot.sp ? (uint32_t)n_slices * per : 0u;
     for (uint32_t e0 = 0; e0 < total;) {
@@ -568,52 +570,47 @@ __global__ __launch_bounds__(NT) void pick_i8_kernel(MaxArgs m)
             // every 256 items, where it did not do
 #pragma unroll 1
             for (int turn = 0;; ++turn) {
-                for (int c0 = 0; c0 < c * CELL; c0 += 256 * ROUNDS) {
+                for (int c0 = 0; c0 < c * CELL; c0 += STEP) {
                     int acc[ROUNDS];
                     int64_t own[ROUNDS];
                     typename RowDot<LPI>::Scale sc[ROUNDS];
-                    if (tid < 256) {
-                        uint4 q[ROUNDS][LPI];
+                    uint4 q[ROUNDS][LPI];
 #pragma unroll
-                        for (int o = 0; o < ROUNDS; ++o) {
-                            const int i = c0 + 256 * o + RowDot<LPI>::owned();
-                            own[o] = i < c * CELL ? cell_item(cand[i / CELL], i % CELL) : a.n_items;
-                            sc[o] = dot.scale(a, own[o] < a.n_items ? own[o] : 0);
-                        }
-#pragma unroll
-                        for (int o = 0; o < ROUNDS; ++o)
-#pragma unroll
-                            for (int j = 0; j < LPI; ++j) {
-                                const int i = c0 + 256 * o + j * (256 / LPI) + tid / LPI;
-                                int64_t it = i < c * CELL ? cell_item(cand[i / CELL], i % CELL) : 0;
-                                it = it < a.n_items ? it : 0;
-                                q[o][j] = dot.load(a, it);
-                            }
-#pragma unroll
-                        for (int o = 0; o < ROUNDS; ++o)
-#pragma unroll
-                            for (int j = 0; j < LPI; ++j) {
-                                const int s = dot.dot(q[o][j]);
-                                if (tid % LPI == j) acc[o] = s;
-                            }
+                    for (int o = 0; o < ROUNDS; ++o) {
+                        const int i = c0 + 256 * (o * TEAMS + team) + RowDot<LPI>::owned();
+                        own[o] = i < c * CELL ? cell_item(cand[i / CELL], i % CELL) : a.n_items;
+                        sc[o] = dot.scale(a, own[o] < a.n_items ? own[o] : 0);
                     }
-                    uint64_t k64[ROUNDS];
-                    if (tid < 256)
 #pragma unroll
-                        for (int o = 0; o < ROUNDS; ++o) {
-                            const float v = dot.score(acc[o], sc[o]);
-                            k64[o] = own[o] < a.n_items && v > -INFINITY ? make_key(v, (int32_t)(id0 + own[o])) : 0;
+                    for (int o = 0; o < ROUNDS; ++o)
+#pragma unroll
+                        for (int j = 0; j < LPI; ++j) {
+                            const int i = c0 + 256 * (o * TEAMS + team) + j * (256 / LPI) + lane_row;
+                            int64_t it = i < c * CELL ? cell_item(cand[i / CELL], i % CELL) : 0;
+                            it = it < a.n_items ? it : 0;
+                            q[o][j] = dot.load(a, it);
                         }
+                    uint64_t k64[ROUNDS];
+#pragma unroll
+                    for (int o = 0; o < ROUNDS; ++o) {
+#pragma unroll
+                        for (int j = 0; j < LPI; ++j) {
+                            const int s = dot.dot(q[o][j]);
+                            if (tid % LPI == j) acc[o] = s;
+                        }
+                        const float v = dot.score(acc[o], sc[o]);
+                        k64[o] = own[o] < a.n_items && v > -INFINITY ? make_key(v, (int32_t)(id0 + own[o])) : 0;
+                    }
                     if (turn == 0) {
                         const uint64_t least = g.kth;
-                        if (tid < 256) group_append_many<ROUNDS>(g, [&](int o) { return k64[o] > least ? k64[o] : 0; });
+                        group_append_many<ROUNDS>(g, [&](int o) { return k64[o] > least ? k64[o] : 0; });
                     } else {
 #pragma unroll 1
-                        for (int o = 0; o < ROUNDS && c0 + 256 * o < c * CELL; ++o) {
+                        for (int t = 0; t < ROUNDS * TEAMS && c0 + 256 * t < c * CELL; ++t) {
                             uint64_t mine = k64[0];
 #pragma unroll
-                            for (int i = 1; i < ROUNDS; ++i) mine = i == o ? k64[i] : mine;
-                            if (tid < 256) group_append(g, mine > g.kth, mine);
+                            for (int i = 1; i < ROUNDS; ++i) mine = i == t / TEAMS ? k64[i] : mine;
+                            if (team == t % TEAMS) group_append(g, mine > g.kth, mine);
                             group_check(g, a.k, a.train_indices, mlo, mhi);
                         }
                     }
