@@ -456,8 +456,8 @@ __device__ __forceinline__ int64_t cell_item(int64_t y, int e) { return cell_fir
 
 // NT = 256 threads, or 1024 where there are few users and one workgroup's time is the call's; LPI: see RowDot.
 // Bound by latency, some twenty dependent steps a user: 4096 users of 200k items 68 to 75 us (five workgroups a CU; more of
-// them at fewer registers gain nothing; with a look at the list's room every 256 items 80), one user of 200k items 15 us, 33
-// of 2M items 25 us.
+// them at fewer registers gain nothing; with a look at the list's room every 256 items 80), one user of 200k items 12.5 us,
+// 33 of 2M items 20 us (with 256 of the 1024 threads scoring 15 and 25).
 template <int NT, int LPI, int LIST>
 __global__ __launch_bounds__(NT) void pick_i8_kernel(MaxArgs m)
 {
@@ -632,7 +632,7 @@ __global__ __launch_bounds__(NT) void pick_i8_kernel(MaxArgs m)
 }
 
 // ------------------------------------------------------------------------------------------
-// few items: a workgroup scores them all for one user, 16 per thread at most (943 users of 1682 items, 20 columns: 16.6 us,
+// few items: a workgroup scores them all for one user, 16 per thread at most (943 users of 1682 items, 20 columns: 13.4 us,
 // nearly all of it the dependent steps of one workgroup)
 // ------------------------------------------------------------------------------------------
 template <int LPI, int LIST>
@@ -649,14 +649,11 @@ __global__ __launch_bounds__(256) void score_small_i8_kernel(ScoreI8Args a)
     dot.init(a, prow);
     const int64_t id0 = a.id_offset + a.item_lo;
     const int n_items = (int)a.n_items, own = RowDot<LPI>::owned();
+    // (the train row is requested ahead of the items and looked at behind them)
+    const int64_t mlo = a.train_indptr ? a.train_indptr[user] : 0, mhi = a.train_indptr ? a.train_indptr[user + 1] : 0;
+    const int32_t train0 = mlo + tid < mhi ? a.train_indices[mlo + tid] : -1;
     for (int i = tid; i < SMALL_ITEMS / 32; i += 256) train[i] = 0;
     if (tid == 0) g.count = 0;
-    __syncthreads();
-    if (a.train_indptr)
-        for (int64_t t = a.train_indptr[user] + tid, e = a.train_indptr[user + 1]; t < e; t += 256) {
-            const int64_t i = a.train_indices[t] - id0;
-            if (i >= 0 && i < n_items) atomicOr(&train[i >> 5], 1u << (i & 31));
-        }
     __syncthreads();
     uint32_t key[V];
     constexpr int BATCH = LPI <= 4 ? 4 : (LPI == 8 ? 2 : 1);           // rounds of 256 items whose rows are requested together
@@ -686,13 +683,33 @@ __global__ __launch_bounds__(256) void score_small_i8_kernel(ScoreI8Args a)
                 if (tid % LPI == j) acc = s;
             }
             const int i = 256 * (v0 + o) + own;
-            if (i < n_items && !(train[i >> 5] >> (i & 31) & 1u)) {
+            if (i < n_items) {
                 const float s = dot.score(acc, sc[o]);
                 key[v0 + o] = s > -INFINITY ? f32_orderable(s) : 0u;
             }
         }
     }
-    const uint32_t cut = rank_bound<256, V>(key, KEY_NONE, a.k, g);
+    auto mark = [&](int32_t id) {
+        const int64_t i = id - id0;
+        if (id >= 0 && i >= 0 && i < n_items) atomicOr(&train[i >> 5], 1u << (i & 31));
+    };
+    mark(train0);
+    for (int64_t t = mlo + tid + 256; t < mhi; t += 256) mark(a.train_indices[t]);
+    __syncthreads();
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        const int i = 256 * v + own;
+        if (train[i >> 5] >> (i & 31) & 1u) key[v] = 0;
+    }
+    // the k-th largest of the threads' best is a lower bound of the k-th largest of all, for few k nearly as high (k = 50: about
+    // 56 keys reach it) and found from one value a thread: 943 users of 1682 items 16.1 -> 13.4 us
+    uint32_t cut;
+    if constexpr (LIST == 512) {
+        uint32_t best[1] = {0};
+#pragma unroll
+        for (int v = 0; v < V; ++v) best[0] = key[v] > best[0] ? key[v] : best[0];
+        cut = rank_bound<256, 1>(best, KEY_NONE, a.k, g);
+    } else cut = rank_bound<256, V>(key, KEY_NONE, a.k, g);
     if (tid == 0) g.kth = cut ? ((uint64_t)cut << 32) - 1 : ((uint64_t)KEY_NONE << 32 | 0xffffffffu);
     __syncthreads();
     // (as in pick_i8_kernel: all keys at once where they fit the list, else 256 at a time)
