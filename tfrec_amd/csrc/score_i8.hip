@@ -455,7 +455,7 @@ __device__ __forceinline__ int64_t cell_first(int64_t y) { return (y >> 1) * BLO
 __device__ __forceinline__ int64_t cell_item(int64_t y, int e) { return cell_first(y) + 8 * (e >> 2) + (e & 3); }
 
 // NT = 256 threads, or 1024 where there are few users and one workgroup's time is the call's; LPI: see RowDot.
-// Bound by latency, some twenty dependent steps a user: 4096 users of 200k items 68 to 75 us (five workgroups a CU; more of
+// Bound by latency, some twenty dependent steps a user: 4096 users of 200k items 68 to 78 us (five workgroups a CU; more of
 // them at fewer registers gain nothing; with a look at the list's room every 256 items 80), one user of 200k items 12.5 us,
 // 33 of 2M items 20 us (with 256 of the 1024 threads scoring 15 and 25).
 template <int NT, int LPI, int LIST>
