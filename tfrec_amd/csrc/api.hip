@@ -22,9 +22,19 @@ int tfrec_ctx_enter(tfrec_ctx *ctx)
     return TFREC_OK;
 }
 
+// Sets *in_graph where the context's stream is being captured: the block in question is then named by a graph.
+static int note_capture(tfrec_ctx *ctx, bool *in_graph)
+{
+    if (*in_graph) return TFREC_OK;
+    hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+    TF_HIP(hipStreamIsCapturing(ctx->stream, &cap));
+    *in_graph = cap != hipStreamCaptureStatusNone;
+    return TFREC_OK;
+}
+
 int tfrec_ws_require(tfrec_ctx *ctx, size_t bytes)
 {
-    if (bytes <= ctx->ws_bytes) return TFREC_OK;
+    if (bytes <= ctx->ws_bytes) return ctx->ws_fixed ? TFREC_OK : note_capture(ctx, &ctx->ws_in_graph);
     TF_REQUIRE(!ctx->ws_fixed, TFREC_ENOMEM, "the fixed scratch block holds %zu bytes, %zu needed", ctx->ws_bytes, bytes);
     // under capture nothing may be waited for or allocated: refused before the capture is spoilt
     hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
@@ -49,15 +59,6 @@ int tfrec_ws_require(tfrec_ctx *ctx, size_t bytes)
         return TFREC_ENOMEM;
     }
     ctx->ws_bytes = want;
-    return TFREC_OK;
-}
-
-int tfrec_note_capture(tfrec_ctx *ctx)
-{
-    if (ctx->ws_in_graph) return TFREC_OK;
-    hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
-    TF_HIP(hipStreamIsCapturing(ctx->stream, &cap));
-    ctx->ws_in_graph = cap != hipStreamCaptureStatusNone;
     return TFREC_OK;
 }
 

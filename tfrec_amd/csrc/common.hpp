@@ -95,12 +95,11 @@ void tfrec_marks_reset(tfrec_ctx *ctx);
 int tfrec_scratch_bind(int device);
 // Makes ctx's device current for the calling thread.
 int tfrec_ctx_enter(tfrec_ctx *ctx);
-// Ensures the workspace holds at least `bytes` (may reallocate: previous carve-outs die).
+// Ensures the workspace holds at least `bytes` (may reallocate: previous carve-outs die).  Every user of the workspace calls
+// it, so it is here that a call under stream capture is noted: the block it names then outlives its replacement.
 int tfrec_ws_require(tfrec_ctx *ctx, size_t bytes);
 // Carves `bytes` (256-byte aligned) out of the workspace; tfrec_ws_require must have covered it.
 void *tfrec_ws_take(tfrec_ctx *ctx, size_t bytes);
-// Called by entry points whose launches may be captured: from then on the workspace's blocks outlive their replacement.
-int tfrec_note_capture(tfrec_ctx *ctx);
 int tfrec_pinned_require(tfrec_ctx *ctx, size_t bytes);
 
 static inline size_t tf_align(size_t x, size_t a = 256) { return (x + a - 1) / a * a; }

@@ -849,7 +849,6 @@ int tfrec_score_i8(tfrec_ctx *ctx, ScoreI8Args a)
     m.pitch = m.groups * 16;
     const int64_t per_pass = users_per_pass(a.n, m.groups);
     TF_TRY(tfrec_ws_require(ctx, ctx->ws_used + tfrec_score_i8_bytes(a.n, a.n_items, a.d, a.k)));
-    TF_TRY(tfrec_note_capture(ctx));
     m.bound = (float *)tfrec_ws_take(ctx, (size_t)per_pass * m.pitch * 4);
     m.group_bound = (float *)tfrec_ws_take(ctx, (size_t)per_pass * m.groups * 4);
     const size_t slack = slack_bytes(per_pass, m.groups, a.d);
