@@ -22,39 +22,53 @@ int tfrec_ctx_enter(tfrec_ctx *ctx)
     return TFREC_OK;
 }
 
-// Sets *in_graph where the context's stream is being captured: the block in question is then named by a graph.
-static int note_capture(tfrec_ctx *ctx, bool *in_graph)
+int tfrec_note_capture(hipStream_t stream, bool *in_graph)
 {
     if (*in_graph) return TFREC_OK;
     hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
-    TF_HIP(hipStreamIsCapturing(ctx->stream, &cap));
+    TF_HIP(hipStreamIsCapturing(stream, &cap));
     *in_graph = cap != hipStreamCaptureStatusNone;
+    return TFREC_OK;
+}
+
+int tfrec_may_grow(hipStream_t stream, const char *what, size_t have, size_t need)
+{
+    hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+    TF_HIP(hipStreamIsCapturing(stream, &cap));
+    TF_REQUIRE(cap == hipStreamCaptureStatusNone, TFREC_ENOMEM,
+               "%s holds %zu bytes, %zu needed: it cannot grow while the stream is captured (make the call once, or reserve, before)", what, have, need);
+    return TFREC_OK;
+}
+
+int tfrec_drop_block(tfrec_ctx *ctx, char **block, bool *in_graph)
+{
+    if (*block && *in_graph) {
+        TF_REQUIRE(ctx->n_retired < (int)(sizeof(ctx->retired) / sizeof(ctx->retired[0])), TFREC_ENOMEM,
+                   "scratch grew too often beside captured graphs: reserve it for the largest call first");
+        ctx->retired[ctx->n_retired++] = *block;
+        *block = nullptr;
+        *in_graph = false;
+    } else if (*block) {
+        TF_HIP(hipFree(*block));
+        *block = nullptr;
+    }
     return TFREC_OK;
 }
 
 int tfrec_ws_require(tfrec_ctx *ctx, size_t bytes)
 {
-    if (bytes <= ctx->ws_bytes) return ctx->ws_fixed ? TFREC_OK : note_capture(ctx, &ctx->ws_in_graph);
+    if (bytes <= ctx->ws_bytes) return ctx->ws_fixed ? TFREC_OK : tfrec_note_capture(ctx->stream, &ctx->ws_in_graph);
     TF_REQUIRE(!ctx->ws_fixed, TFREC_ENOMEM, "the fixed scratch block holds %zu bytes, %zu needed", ctx->ws_bytes, bytes);
     // under capture nothing may be waited for or allocated: refused before the capture is spoilt
-    hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
-    TF_HIP(hipStreamIsCapturing(ctx->stream, &cap));
-    TF_REQUIRE(cap == hipStreamCaptureStatusNone, TFREC_ENOMEM,
-               "the workspace holds %zu bytes, %zu needed: it cannot grow while the stream is captured (call tfrec_ctx_reserve, or the entry once, before)",
-               ctx->ws_bytes, bytes);
+    TF_TRY(tfrec_may_grow(ctx->stream, "the workspace", ctx->ws_bytes, bytes));
     // grow: wait for work that may still use the old block, then replace it (a block that a captured graph names is kept)
     TF_HIP(hipStreamSynchronize(ctx->stream));
-    if (ctx->ws && ctx->ws_in_graph) {
-        TF_REQUIRE(ctx->n_retired < (int)(sizeof(ctx->retired) / sizeof(ctx->retired[0])), TFREC_ENOMEM,
-                   "the workspace grew too often beside captured graphs: reserve it for the largest call first");
-        ctx->retired[ctx->n_retired++] = ctx->ws;
-        ctx->ws_in_graph = false;
-    } else if (ctx->ws) TF_HIP(hipFree(ctx->ws));
-    ctx->ws = nullptr;
+    TF_TRY(tfrec_drop_block(ctx, &ctx->ws, &ctx->ws_in_graph));
     ctx->ws_bytes = 0;
     const size_t want = tf_align(bytes + bytes / 8, 1 << 20);
     hipError_t e = hipMalloc((void **)&ctx->ws, want);
     if (e != hipSuccess) {
+        ctx->ws = nullptr;
         tfrec_set_error("workspace allocation of %zu bytes failed: %s", want, hipGetErrorString(e));
         return TFREC_ENOMEM;
     }

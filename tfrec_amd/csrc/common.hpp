@@ -45,6 +45,7 @@ void tfrec_set_error(const char *fmt, ...);
 struct tfrec_batch_slot {
     char *mem = nullptr;
     size_t bytes = 0;
+    bool in_graph = false;                   // a captured call uses the block: it then stays until the context is destroyed
     int64_t B = -1, U = 0, I = 0;            // B < 0: nothing prepared
     int K = 1, next_k = 0;                   // batches sorted together / next one to consume
     uint32_t kmask = 0xffffffffu;            // key bits below the batch number
@@ -65,7 +66,7 @@ struct tfrec_ctx {
     size_t ws_bytes = 0;
     size_t ws_used = 0;          // bump pointer, reset at the start of every entry point
     bool ws_in_graph = false;    // a call that was captured into a HIP graph uses the workspace: its blocks then stay until destroy
-    void *retired[16] = {};      // blocks the workspace grew out of while a graph may still name them
+    void *retired[16] = {};      // blocks the workspace and the batch slots grew out of while a graph may still name them
     int n_retired = 0;
     char *d_small = nullptr;     // TFREC_SMALL_BYTES of scratch that never moves (partial sums of the gradient norm)
     bool ws_fixed = false;       // the workspace is a borrowed block of fixed size: never grown, never freed
@@ -100,6 +101,11 @@ int tfrec_ctx_enter(tfrec_ctx *ctx);
 int tfrec_ws_require(tfrec_ctx *ctx, size_t bytes);
 // Carves `bytes` (256-byte aligned) out of the workspace; tfrec_ws_require must have covered it.
 void *tfrec_ws_take(tfrec_ctx *ctx, size_t bytes);
+// The same for scratch outside the workspace (the batch slots): *in_graph is set where `stream` is being captured, growth is
+// refused there, and a block that is grown out of is freed, or kept until the context is destroyed if *in_graph.
+int tfrec_note_capture(hipStream_t stream, bool *in_graph);
+int tfrec_may_grow(hipStream_t stream, const char *what, size_t have, size_t need);
+int tfrec_drop_block(tfrec_ctx *ctx, char **block, bool *in_graph);
 int tfrec_pinned_require(tfrec_ctx *ctx, size_t bytes);
 
 static inline size_t tf_align(size_t x, size_t a = 256) { return (x + a - 1) / a * a; }

@@ -657,15 +657,16 @@ static int slot_prepare(tfrec_ctx *ctx, tfrec_batch_slot &sl, hipStream_t stream
     size_t sort_bytes = 0;
     const size_t need = slot_bytes(n, &sort_bytes);
     if (need > sl.bytes) {
+        TF_TRY(tfrec_may_grow(stream, "the batch slot", sl.bytes, need));
         // growing: nothing may still be reading the old block
         TF_HIP(hipStreamSynchronize(ctx->stream));
         if (ctx->aux_stream) TF_HIP(hipStreamSynchronize(ctx->aux_stream));
-        if (sl.mem) TF_HIP(hipFree(sl.mem));
-        sl.mem = nullptr; sl.bytes = 0;
+        TF_TRY(tfrec_drop_block(ctx, &sl.mem, &sl.in_graph));
+        sl.bytes = 0;
         hipError_t e = hipMalloc((void **)&sl.mem, need + need / 8);
-        if (e != hipSuccess) { tfrec_set_error("batch slot allocation of %zu bytes failed: %s", need, hipGetErrorString(e)); return TFREC_ENOMEM; }
+        if (e != hipSuccess) { sl.mem = nullptr; tfrec_set_error("batch slot allocation of %zu bytes failed: %s", need, hipGetErrorString(e)); return TFREC_ENOMEM; }
         sl.bytes = need + need / 8;
-    }
+    } else if (!ctx->ws_fixed) TF_TRY(tfrec_note_capture(stream, &sl.in_graph));
     char *p = sl.mem;
     auto take = [&](size_t bytes) { char *r = p; p += tf_align(bytes); return r; };
     sl.keys = (uint32_t *)take(12 * (size_t)n);
@@ -1309,18 +1310,28 @@ extern "C" int tfrec_bpr_grads(tfrec_ctx *ctx, const float *d_P, const float *d_
     }
     TF_TRY(tfrec_ctx_enter(ctx));
     TF_TRY(check_step_args(d_P, d_Q, d_b, U, I, d, d_users, d_pos, d_neg, B));
-    zero_tables_kernel<<<2048, 256, 0, ctx->stream>>>(d_gP, U * d, d_gQ, I * d, d_gb, I);
-    TF_HIP(hipGetLastError());
+    auto zero = [&]() -> int {
+        zero_tables_kernel<<<2048, 256, 0, ctx->stream>>>(d_gP, U * d, d_gQ, I * d, d_gb, I);
+        TF_HIP(hipGetLastError());
+        return TFREC_OK;
+    };
     if (B == 0) {
+        TF_TRY(zero());
         if (d_loss) zero_tables_kernel<<<1, 256, 0, ctx->stream>>>((float *)d_loss, 4, nullptr, 0, nullptr, 0);
         TF_HIP(hipGetLastError());
         return TFREC_OK;
     }
+    // all scratch is there before the first launch: a captured call that is refused for it has recorded nothing
+    RowCfg cfg;
+    TF_REQUIRE(pick_cfg(d, all_aligned16({d_P, d_Q, d_gP, d_gQ}), &cfg), TFREC_EUNSUP, "factor size d=%d is not supported (max 256)", d);
+    TF_TRY(tfrec_ws_require(ctx, step_ws_bytes(B, d, cfg)));
     tfrec_marks_reset(ctx);
     tfrec_mark(ctx, "start");
     tfrec_batch_slot &sl = ctx->slots[2];
     TF_TRY(slot_prepare(ctx, sl, ctx->stream, d_users, d_pos, d_neg, B, U, I));
     tfrec_mark(ctx, "index");
+    TF_TRY(zero());
+    tfrec_mark(ctx, "zero");
     return bpr_passes(ctx, sl, const_cast<float *>(d_P), const_cast<float *>(d_Q), const_cast<float *>(d_b), U, d, 0.f, reg, d_loss, true, d_gQ, d_gb,
                       nullptr, nullptr, d_gP);
 }
