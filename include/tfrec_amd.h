@@ -338,15 +338,14 @@ int tfrec_bpr_grads(tfrec_ctx *ctx, const float *d_P, const float *d_Q, const fl
  * at any alignment of its type.  A tensor listed twice counts twice.  The host arrays are read before the call returns.
  * No counterpart in the reference (tf.train optimizers step on what they get, model/BPR.py:48). */
 int tfrec_grad_norm(tfrec_ctx *ctx, int n, const void *const *h_grads, const int64_t *h_counts, const int *h_dtypes, float *d_norm);
-/* The same, and h_out[i] = h_grads[i] * s with s = max_norm / max(norm, max_norm), formed in float64 and rounded to
- * float32; the product is rounded to float32, then to the tensor's type.  Within the bound s is 1 and every value is
- * left as it is.  A norm that is infinite or not a number makes every value NaN.  h_out[i] may be
+/* The same, and h_out[i] = h_grads[i] * s with s = max_norm / max(norm, max_norm) held beyond float32's bits (max_norm and norm
+ * in float64); the product is rounded to float32, then to the tensor's type.  Within the bound s is 1 and every value is left as it is.  A norm that is infinite or not a number makes every value NaN.  h_out[i] may be
  * h_grads[i]; apart from that no output may overlap another output or any gradient (TFREC_EINVAL).  d_norm (the norm
  * before scaling) may be null.  max_norm: positive and finite.
  * These calls use fixed scratch of the context, never its workspace, and can be captured into a HIP graph; graphs
  * captured from one context share that scratch and must not be replayed at the same time. */
 int tfrec_grad_clip(tfrec_ctx *ctx, int n, const void *const *h_grads, void *const *h_out, const int64_t *h_counts,
-                    const int *h_dtypes, float max_norm, float *d_norm);
+                    const int *h_dtypes, double max_norm, float *d_norm);
 
 /* The same on a list that is kept: a program that steps on the same gradient buffers makes one list, and a step is then
  * one launch for a few ten thousand values and two for any other number, whatever the number of tensors.
@@ -358,7 +357,7 @@ int tfrec_grads_create(tfrec_ctx *ctx, int n, const void *const *h_grads, void *
                        const int *h_dtypes, tfrec_grads **out);
 int tfrec_grads_destroy(tfrec_ctx *ctx, tfrec_grads *g);
 int tfrec_grads_norm(tfrec_ctx *ctx, const tfrec_grads *g, float *d_norm);
-int tfrec_grads_clip(tfrec_ctx *ctx, const tfrec_grads *g, float max_norm, float *d_norm);
+int tfrec_grads_clip(tfrec_ctx *ctx, const tfrec_grads *g, double max_norm, float *d_norm);
 
 /* ---- 8-bit rows ------------------------------------------------------------------------------- */
 /* A matrix in 8-bit integers with one float32 scale per row: value = q * scale.  Rows are ldq bytes apart, ldq a

@@ -20,6 +20,7 @@ _p = C.c_void_p
 _i64 = C.c_int64
 _int = C.c_int
 _f = C.c_float
+_d = C.c_double
 _u64 = C.c_uint64
 
 # name -> (restype, argtypes); one entry per symbol declared in include/tfrec_amd.h
@@ -72,11 +73,11 @@ SIGNATURES = {
     "tfrec_bpr_dense_grad_step": (_int, [_p, _int, _p, _p, _p, _p, _i64, _i64, _int, _p, _p, _p, _i64, _f, _f, _p]),
     "tfrec_bpr_grads": (_int, [_p, _p, _p, _p, _i64, _i64, _int, _p, _p, _p, _i64, _f, _p, _p, _p, _p]),
     "tfrec_grad_norm": (_int, [_p, _int, _p, _p, _p, _p]),
-    "tfrec_grad_clip": (_int, [_p, _int, _p, _p, _p, _p, _f, _p]),
+    "tfrec_grad_clip": (_int, [_p, _int, _p, _p, _p, _p, _d, _p]),
     "tfrec_grads_create": (_int, [_p, _int, _p, _p, _p, _p, C.POINTER(_p)]),
     "tfrec_grads_destroy": (_int, [_p, _p]),
     "tfrec_grads_norm": (_int, [_p, _p, _p]),
-    "tfrec_grads_clip": (_int, [_p, _p, _f, _p]),
+    "tfrec_grads_clip": (_int, [_p, _p, _d, _p]),
     "tfrec_quantize_rows_i8": (_int, [_p, _p, _int, _i64, _i64, _i64, _p, _i64, _p, _i64, _p]),
     "tfrec_matmul_i8": (_int, [_p, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _i64, _p, _p, _int, _i64]),
     "tfrec_score_topk_i8": (_int, [_p, _p, _i64, _p, _i64, _int, _p, _i64, _p, _p, _i64, _int, _i64, _i64, _p, _i64, _p, _p, _int, _p, _p]),

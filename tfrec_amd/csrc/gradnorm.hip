@@ -82,8 +82,36 @@ __device__ __forceinline__ double chunk_squares(const T *__restrict__ x, int m, 
     return s;
 }
 
-template <class T>
-__device__ __forceinline__ void chunk_scale(const T *x, T *y, int m, float s, float p2)
+// The factor s of every value: max_norm / norm in float64, as hi + lo in float32.  hi alone would cost a second half step;
+// fma(x, hi, x * lo) is x s rounded once (lo is within 2^-48 of what hi leaves; next to the subnormal numbers x * lo may be half a
+// step off), in two instructions.  Factors below 2^-76, whose lo could leave float32's range (bounds of 1e-38 beside gradients of
+// 1e30), take the product in float64; all values that way cost 40 MB of bfloat16 in 600 tensors 23.4 us against 22.2.
+// A sum of squares of finite float32 values stays finite in float64: a norm that is not finite means an infinity or NaN among the
+// values.
+struct GradFactor {
+    double s;
+    float hi, lo;
+    __device__ __forceinline__ GradFactor(double norm, double max_norm)
+    {
+        s = !(norm < (double)INFINITY) ? (double)NAN : (norm <= max_norm ? 1. : max_norm / norm);
+        hi = (float)s;
+        lo = (float)(s - (double)hi);
+    }
+    // in place and within the bound: every value is what it was
+    __device__ __forceinline__ bool nothing(const GradChunk &c) const { return s == 1. && c.src == c.dst; }
+    // calls f(scale) with the form of the product, the same for all values
+    template <class F>
+    __device__ __forceinline__ void with(F &&f) const
+    {
+        const float h = hi, l = lo;
+        const double d = s;
+        if (d < 0x1p-76) f([=](float x) { return (float)((double)x * d); });
+        else f([=](float x) { return fmaf(x, h, x * l); });
+    }
+};
+
+template <class T, class Scale>
+__device__ __forceinline__ void chunk_scale(const T *x, T *y, int m, Scale &&f)
 {
     constexpr int V = 16 / sizeof(T), R = GRAD_CHUNK / (256 * V);
     if (m == GRAD_CHUNK) {
@@ -93,11 +121,11 @@ __device__ __forceinline__ void chunk_scale(const T *x, T *y, int m, float s, fl
 #pragma unroll
         for (int r = 0; r < R; ++r) {
 #pragma unroll
-            for (int j = 0; j < V; ++j) p[r].v[j] = (T)((float)p[r].v[j] * s * p2);
+            for (int j = 0; j < V; ++j) p[r].v[j] = (T)f((float)p[r].v[j]);
             reinterpret_cast<Pack<T> *>(y)[r * 256 + threadIdx.x] = p[r];
         }
     } else {
-        for (int i = threadIdx.x; i < m; i += 256) y[i] = (T)((float)x[i] * s * p2);
+        for (int i = threadIdx.x; i < m; i += 256) y[i] = (T)f((float)x[i]);
     }
 }
 
@@ -115,22 +143,6 @@ __device__ __forceinline__ double block_sum(double v)
     __syncthreads();
     return v;
 }
-
-// The factor of every value, as s * p2.  (A sum of squares of finite float32 values stays finite in float64: a norm that is
-// not finite means an infinity or NaN among the values.)  A factor near or below the subnormal range of float32 (gradients
-// of 1e35 and more) is applied as s 2^64 and then 2^-64.
-struct GradFactor {
-    float s, p2;
-    __device__ __forceinline__ GradFactor(double norm, double max_norm)
-    {
-        const double f = norm <= max_norm ? 1. : max_norm / norm;
-        const bool tiny = f < 0x1p-100;
-        s = !(norm < (double)INFINITY) ? NAN : (float)(tiny ? f * 0x1p64 : f);
-        p2 = tiny ? 0x1p-64f : 1.f;
-    }
-    // in place and within the bound: every value is what it was
-    __device__ __forceinline__ bool nothing(const GradChunk &c) const { return s == 1.f && c.src == c.dst; }
-};
 
 // 308 MB of float32 in 3 tensors: 77 us, 4.0 TB/s, what a plain sum of them reads; 40 MB of bfloat16 in 600 tensors 16 us
 // (both from the caches in part).  2048 workgroups: 4096 take 14 us and their norm 1 us more, 1024 take 21 us.
@@ -169,10 +181,12 @@ __global__ __launch_bounds__(256) void grad_scale_kernel(Table t, const double *
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)nm;
     const GradFactor f(nm, max_norm);
     // the last chunks first: what the norm read last is still cached
-    for (int64_t k = blockIdx.x; k < t.chunks; k += gridDim.x) {
-        const GradChunk c = t.get(t.chunks - 1 - k);
-        if (!f.nothing(c)) by_type(c, [&]<class T>(const T *x, T *y) { chunk_scale(x, y, c.len, f.s, f.p2); });
-    }
+    f.with([&](auto &&scale) {
+        for (int64_t k = blockIdx.x; k < t.chunks; k += gridDim.x) {
+            const GradChunk c = t.get(t.chunks - 1 - k);
+            if (!f.nothing(c)) by_type(c, [&]<class T>(const T *x, T *y) { chunk_scale(x, y, c.len, scale); });
+        }
+    });
 }
 
 // Few values: one workgroup holds all of them in registers between the norm and the product (one launch, one read).
@@ -221,26 +235,28 @@ __global__ __launch_bounds__(1024) void grad_clip_small_kernel(Table t, double m
     const double nm = sqrt(block_sum<16>(s));
     if (norm && threadIdx.x == 0) *norm = (float)nm;
     const GradFactor f(nm, max_norm);
+    f.with([&](auto &&scale) {
 #pragma unroll
-    for (int k = 0; k < GRAD_SMALL; ++k) {
-        if (k >= n) break;
-        const GradChunk &c = cs[k];
-        if (f.nothing(c)) continue;
-        by_type(c, [&]<class T>(const T *, T *y) {
-            constexpr int V = 16 / sizeof(T), R = 8 / V;
+        for (int k = 0; k < GRAD_SMALL; ++k) {
+            if (k >= n) break;
+            const GradChunk &c = cs[k];
+            if (f.nothing(c)) continue;
+            by_type(c, [&]<class T>(const T *, T *y) {
+                constexpr int V = 16 / sizeof(T), R = 8 / V;
 #pragma unroll
-            for (int r = 0; r < R; ++r) {
-                const int i = (r * 1024 + threadIdx.x) * V;
-                Pack<T> p = __builtin_bit_cast(Pack<T>, held[k][r]);
+                for (int r = 0; r < R; ++r) {
+                    const int i = (r * 1024 + threadIdx.x) * V;
+                    Pack<T> p = __builtin_bit_cast(Pack<T>, held[k][r]);
 #pragma unroll
-                for (int j = 0; j < V; ++j) p.v[j] = (T)((float)p.v[j] * f.s * f.p2);
-                if (i + V <= c.len) *reinterpret_cast<Pack<T> *>(y + i) = p;
-                else
-                    for (int j = 0; j < V; ++j)
-                        if (i + j < c.len) y[i + j] = p.v[j];
-            }
-        });
-    }
+                    for (int j = 0; j < V; ++j) p.v[j] = (T)scale((float)p.v[j]);
+                    if (i + V <= c.len) *reinterpret_cast<Pack<T> *>(y + i) = p;
+                    else
+                        for (int j = 0; j < V; ++j)
+                            if (i + j < c.len) y[i + j] = p.v[j];
+                }
+            });
+        }
+    });
 }
 
 static inline size_t dt_size(int t) { return t == TFREC_DT_F32 ? 4 : 2; }
@@ -358,11 +374,11 @@ static int run_norm(tfrec_ctx *ctx, int64_t most, Each &&each, int *n_part)
 }
 
 template <class Each>
-static int run_clip(tfrec_ctx *ctx, int64_t most, int tables, Each &&each, float max_norm, float *d_norm)
+static int run_clip(tfrec_ctx *ctx, int64_t most, int tables, Each &&each, double max_norm, float *d_norm)
 {
     if (tables == 1 && most <= GRAD_SMALL)
         return each([&](const auto &t) -> int {
-            grad_clip_small_kernel<<<1, 1024, 0, ctx->stream>>>(t, (double)max_norm, d_norm);
+            grad_clip_small_kernel<<<1, 1024, 0, ctx->stream>>>(t, max_norm, d_norm);
             TF_HIP(hipGetLastError());
             return TFREC_OK;
         });
@@ -372,7 +388,7 @@ static int run_clip(tfrec_ctx *ctx, int64_t most, int tables, Each &&each, float
     bool any = false;
     TF_TRY(each([&](const auto &t) -> int {
         const int blocks = t.chunks < 2048 ? (int)t.chunks : 2048;
-        grad_scale_kernel<<<blocks, 256, 0, ctx->stream>>>(t, part, n_part, (double)max_norm, any ? nullptr : d_norm);
+        grad_scale_kernel<<<blocks, 256, 0, ctx->stream>>>(t, part, n_part, max_norm, any ? nullptr : d_norm);
         TF_HIP(hipGetLastError());
         any = true;
         return TFREC_OK;
@@ -391,9 +407,9 @@ static int finish_norm(tfrec_ctx *ctx, int n_part, float *d_norm)
     return TFREC_OK;
 }
 
-static int check_bound(float max_norm, const float *d_norm)
+static int check_bound(double max_norm, const float *d_norm)
 {
-    TF_REQUIRE(max_norm > 0.f && max_norm < INFINITY, TFREC_EINVAL, "max_norm must be positive and finite, got %g", (double)max_norm);
+    TF_REQUIRE(max_norm > 0. && max_norm < (double)INFINITY, TFREC_EINVAL, "max_norm must be positive and finite, got %g", max_norm);
     TF_REQUIRE(((uintptr_t)d_norm & 3u) == 0, TFREC_EINVAL, "misaligned output");
     return TFREC_OK;
 }
@@ -412,7 +428,7 @@ extern "C" int tfrec_grad_norm(tfrec_ctx *ctx, int n, const void *const *h_grads
 }
 
 extern "C" int tfrec_grad_clip(tfrec_ctx *ctx, int n, const void *const *h_grads, void *const *h_out, const int64_t *h_counts,
-                               const int *h_dtypes, float max_norm, float *d_norm)
+                               const int *h_dtypes, double max_norm, float *d_norm)
 {
     TF_TRY(check_grads(n, h_grads, h_counts, h_dtypes));
     TF_TRY(check_bound(max_norm, d_norm));
@@ -508,7 +524,7 @@ extern "C" int tfrec_grads_norm(tfrec_ctx *ctx, const tfrec_grads *g, float *d_n
     return finish_norm(ctx, n_part, d_norm);
 }
 
-extern "C" int tfrec_grads_clip(tfrec_ctx *ctx, const tfrec_grads *g, float max_norm, float *d_norm)
+extern "C" int tfrec_grads_clip(tfrec_ctx *ctx, const tfrec_grads *g, double max_norm, float *d_norm)
 {
     TF_REQUIRE(g != nullptr, TFREC_EINVAL, "null list");
     TF_TRY(check_bound(max_norm, d_norm));
