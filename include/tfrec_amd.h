@@ -341,7 +341,7 @@ int tfrec_grad_norm(tfrec_ctx *ctx, int n, const void *const *h_grads, const int
 /* The same, and h_out[i] = h_grads[i] * s with s = max_norm / max(norm, max_norm) held beyond float32's bits (max_norm and norm
  * in float64); the product is rounded to float32, then to the tensor's type.  Within the bound s is 1 and every value is left as it is.  A norm that is infinite or not a number makes every value NaN.  h_out[i] may be
  * h_grads[i]; apart from that no output may overlap another output or any gradient (TFREC_EINVAL).  d_norm (the norm
- * before scaling) may be null.  max_norm: positive and finite.
+ * before scaling) may be null, and may be no part of a gradient or an output.  max_norm: positive and finite.
  * These calls use fixed scratch of the context, never its workspace, and can be captured into a HIP graph; graphs
  * captured from one context share that scratch and must not be replayed at the same time. */
 int tfrec_grad_clip(tfrec_ctx *ctx, int n, const void *const *h_grads, void *const *h_out, const int64_t *h_counts,

@@ -77,3 +77,23 @@ def test_bounds_beyond_the_range_of_float32(dev):
         assert torch.equal(got[0], x)
     for _, got, n in clip_all_ways(dev, [x], 1e-60):
         assert not got[0].any()
+
+
+def test_a_norm_within_a_kept_tensor_is_refused(dev):
+    """The norm of a list may lie anywhere but in a gradient or an output of it."""
+    flat, to = torch.ones(3000, device="cuda"), torch.ones(3000, device="cuda")
+    for out in (None, [to[0:500], to[800:900], to[1000:2000]]):
+        lst = dev.grad_list([flat[0:500], flat[400:500], flat[1000:2000]] if out else [flat[0:500], flat[500:600], flat[1000:2000]], out=out)
+        inside = [flat[0:1], flat[499:500], flat[1000:1001], flat[1999:2000]] + ([to[0:1], to[800:801], to[1999:2000]] if out else [flat[599:600]])
+        for norm in inside:
+            before = flat.clone(), to.clone()
+            with pytest.raises(ValueError, match="norm"):
+                dev.clip_grads(lst, 1.0, norm=norm)
+            dev.synchronize()
+            assert torch.equal(before[0], flat) and torch.equal(before[1], to)
+        outside = [flat[700:701], flat[999:1000], flat[2000:2001], to[500:501] if out else to[0:1]]
+        for norm in outside:
+            dev.clip_grads(lst, 1e6, norm=norm)
+            dev.synchronize()
+            assert float(norm) > 1.0
+            norm.fill_(1.0)

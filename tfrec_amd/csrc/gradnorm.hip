@@ -274,13 +274,26 @@ static int check_grads(int n, const void *const *g, const int64_t *counts, const
     return TFREC_OK;
 }
 
-struct Range { uintptr_t lo, hi; int out; };       // out: index of the output, or -1 for a gradient
+struct Range { uintptr_t lo, hi; int out; };       // out: index of the output
+
+// by address (no library sort: nothing here may throw)
+template <class R>
+static void sort_ranges(R *r, size_t m)
+{
+    for (size_t gap = m / 2; gap > 0; gap /= 2)
+        for (size_t i = gap; i < m; ++i) {
+            const R x = r[i];
+            size_t j = i;
+            for (; j >= gap && r[j - gap].lo > x.lo; j -= gap) r[j] = r[j - gap];
+            r[j] = x;
+        }
+}
 
 // No output overlaps another output, or a gradient other than the one it replaces.
 static int check_outputs(int n, const void *const *g, void *const *out, const int64_t *counts, const int *dtypes)
 {
     TF_REQUIRE(n == 0 || out, TFREC_EINVAL, "null host array");
-    Range *r = new (std::nothrow) Range[2 * (size_t)n + 1];
+    Range *r = new (std::nothrow) Range[(size_t)n + 1];
     TF_REQUIRE(r != nullptr, TFREC_ENOMEM, "host allocation failed");
     size_t m = 0;
     int bad = -1, why = 0;
@@ -297,13 +310,7 @@ static int check_outputs(int n, const void *const *g, void *const *out, const in
     if (bad < 0) {
         // outputs by address, then every gradient against the outputs around it
         if (!sorted) {
-            for (size_t gap = m / 2; gap > 0; gap /= 2)            // (no library sort: nothing here may throw)
-                for (size_t i = gap; i < m; ++i) {
-                    const Range x = r[i];
-                    size_t j = i;
-                    for (; j >= gap && r[j - gap].lo > x.lo; j -= gap) r[j] = r[j - gap];
-                    r[j] = x;
-                }
+            sort_ranges(r, m);
             for (size_t i = 1; i < m; ++i)
                 if (r[i - 1].hi > r[i].lo) { bad = r[i].out; why = 3; break; }
         }
@@ -322,6 +329,19 @@ static int check_outputs(int n, const void *const *g, void *const *out, const in
     delete[] r;
     TF_REQUIRE(bad < 0, TFREC_EINVAL, why == 1 ? "output %d is null" : why == 2 ? "output %d is not aligned to its type"
                : why == 3 ? "output %d overlaps another output" : "output %d overlaps a gradient that it does not replace", bad);
+    return TFREC_OK;
+}
+
+// The norm is written while gradients are still read and outputs written: it may be no part of either.
+static int check_norm_apart(int n, const void *const *g, void *const *out, const int64_t *counts, const int *dtypes, const float *d_norm)
+{
+    if (!d_norm) return TFREC_OK;
+    const uintptr_t lo = (uintptr_t)d_norm, hi = lo + sizeof(float);
+    for (int i = 0; i < n; ++i) {
+        const size_t bytes = (size_t)counts[i] * dt_size(dtypes[i]);
+        for (const void *p : {g[i], (const void *)out[i]})
+            TF_REQUIRE(bytes == 0 || hi <= (uintptr_t)p || (uintptr_t)p + bytes <= lo, TFREC_EINVAL, "the norm lies within tensor %d", i);
+    }
     return TFREC_OK;
 }
 
@@ -433,6 +453,7 @@ extern "C" int tfrec_grad_clip(tfrec_ctx *ctx, int n, const void *const *h_grads
     TF_TRY(check_grads(n, h_grads, h_counts, h_dtypes));
     TF_TRY(check_bound(max_norm, d_norm));
     TF_TRY(check_outputs(n, h_grads, h_out, h_counts, h_dtypes));
+    TF_TRY(check_norm_apart(n, h_grads, h_out, h_counts, h_dtypes, d_norm));
     TF_TRY(tfrec_ctx_enter(ctx));
     auto each = [&](auto &&f) -> int { return for_tables(n, h_grads, h_out, h_counts, h_dtypes, f); };
     int64_t most = 0;
@@ -444,11 +465,22 @@ extern "C" int tfrec_grad_clip(tfrec_ctx *ctx, int n, const void *const *h_grads
 // ------------------------------------------------------------------------------------------
 // kept lists
 // ------------------------------------------------------------------------------------------
+struct Span { uintptr_t lo, hi; };
+
 struct tfrec_grads {
     GradChunk *d_chunks = nullptr;
     int64_t chunks = 0;
     int device = 0;
+    Span *spans = nullptr;                     // the memory of all gradients and outputs: disjoint, by address
+    size_t n_spans = 0;
 };
+
+static void free_grads(tfrec_grads *g)
+{
+    if (g->d_chunks) (void)hipFree(g->d_chunks);
+    delete[] g->spans;
+    delete g;
+}
 
 extern "C" int tfrec_grads_create(tfrec_ctx *ctx, int n, const void *const *h_grads, void *const *h_out, const int64_t *h_counts,
                                   const int *h_dtypes, tfrec_grads **out)
@@ -465,19 +497,32 @@ extern "C" int tfrec_grads_create(tfrec_ctx *ctx, int n, const void *const *h_gr
     for (int i = 0; i < n; ++i) chunks += (h_counts[i] + GRAD_CHUNK - 1) / GRAD_CHUNK;
     tfrec_grads *g = new (std::nothrow) tfrec_grads();
     GradChunk *h = new (std::nothrow) GradChunk[(size_t)chunks + 1];
-    if (!g || !h) {
-        delete g;
+    if (g) g->spans = new (std::nothrow) Span[2 * (size_t)n + 1];
+    if (!g || !h || !g->spans) {
+        if (g) free_grads(g);
         delete[] h;
         tfrec_set_error("host allocation failed");
         return TFREC_ENOMEM;
     }
     int64_t c = 0;
-    for (int i = 0; i < n; ++i)
+    size_t m = 0;
+    for (int i = 0; i < n; ++i) {
+        const size_t es = dt_size(h_dtypes[i]);
         for (int64_t at = 0; at < h_counts[i]; at += GRAD_CHUNK) {
-            const size_t es = dt_size(h_dtypes[i]);
             const int64_t left = h_counts[i] - at;
             h[c++] = GradChunk{(const char *)h_grads[i] + at * es, (char *)h_out[i] + at * es, (int32_t)(left < GRAD_CHUNK ? left : GRAD_CHUNK), h_dtypes[i], 0};
         }
+        if (!h_counts[i]) continue;
+        g->spans[m++] = {(uintptr_t)h_grads[i], (uintptr_t)h_grads[i] + (size_t)h_counts[i] * es};
+        if (h_out[i] != h_grads[i]) g->spans[m++] = {(uintptr_t)h_out[i], (uintptr_t)h_out[i] + (size_t)h_counts[i] * es};
+    }
+    sort_ranges(g->spans, m);
+    for (size_t i = 0; i < m; ++i) {           // (gradients may overlap each other)
+        if (g->n_spans && g->spans[i].lo <= g->spans[g->n_spans - 1].hi) {
+            Span &last = g->spans[g->n_spans - 1];
+            last.hi = g->spans[i].hi > last.hi ? g->spans[i].hi : last.hi;
+        } else g->spans[g->n_spans++] = g->spans[i];
+    }
     g->chunks = chunks;
     g->device = ctx->device;
     hipError_t e = hipMalloc((void **)&g->d_chunks, sizeof(GradChunk) * (size_t)(chunks > 0 ? chunks : 1));
@@ -487,8 +532,7 @@ extern "C" int tfrec_grads_create(tfrec_ctx *ctx, int n, const void *const *h_gr
     delete[] h;
     if (e != hipSuccess) {
         const int code = g->d_chunks ? TFREC_EHIP : TFREC_ENOMEM;
-        if (g->d_chunks) (void)hipFree(g->d_chunks);
-        delete g;
+        free_grads(g);
         tfrec_set_error("the list of %lld chunks could not be stored: %s", (long long)chunks, hipGetErrorString(e));
         return code;
     }
@@ -502,8 +546,20 @@ extern "C" int tfrec_grads_destroy(tfrec_ctx *ctx, tfrec_grads *g)
     (void)hipSetDevice(g->device);
     if (ctx) (void)hipStreamSynchronize(ctx->stream);
     else (void)hipDeviceSynchronize();
-    if (g->d_chunks) (void)hipFree(g->d_chunks);
-    delete g;
+    free_grads(g);
+    return TFREC_OK;
+}
+
+// check_norm_apart for a kept list
+static int check_norm_outside(const tfrec_grads *g, const float *d_norm)
+{
+    const uintptr_t lo = (uintptr_t)d_norm;
+    size_t a = 0, b = g->n_spans;              // first span that ends behind the norm's first byte
+    while (a < b) {
+        const size_t mid = (a + b) / 2;
+        if (g->spans[mid].hi <= lo) a = mid + 1; else b = mid;
+    }
+    TF_REQUIRE(!d_norm || a == g->n_spans || g->spans[a].lo >= lo + sizeof(float), TFREC_EINVAL, "the norm lies within a tensor of the list");
     return TFREC_OK;
 }
 
@@ -530,6 +586,7 @@ extern "C" int tfrec_grads_clip(tfrec_ctx *ctx, const tfrec_grads *g, double max
     TF_TRY(check_bound(max_norm, d_norm));
     TF_TRY(tfrec_ctx_enter(ctx));
     TF_TRY(check_list(ctx, g));
+    TF_TRY(check_norm_outside(g, d_norm));
     if (g->chunks == 0 && !d_norm) return TFREC_OK;
     return run_clip(ctx, g->chunks, 1, [&](auto &&f) -> int { return f(GradListed{g->d_chunks, g->chunks}); }, max_norm, d_norm);
 }
