@@ -367,14 +367,14 @@ int tfrec_grads_clip(tfrec_ctx *ctx, const tfrec_grads *g, double max_norm, floa
  * to even, in [-127, 127]; columns d .. (d rounded up to 16) are set to 0.  A row of zeros has scale 0; a row that holds
  * an infinity or NaN has scale NaN and zeros.  Source rows of type x_dtype (TFREC_DT_*), ldx elements apart: row
  * d_rows[r] (ids below n_rows; an id outside is clamped and raises the bad-index flag), or row r where d_rows is null
- * (n <= n_rows). */
+ * (n <= n_rows).  The outputs may share no byte with each other, the source rows or the list. */
 int tfrec_quantize_rows_i8(tfrec_ctx *ctx, const void *d_X, int x_dtype, int64_t n_rows, int64_t ldx, int64_t d,
                            const int32_t *d_rows, int64_t n, int8_t *d_q, int64_t ldq, float *d_scale);
 /* C[m, n] = (sum_k A[m, k] B[n, k]) * sa[m] * sb[n] + bias[n] (d_bias may be null): the 8-bit form of the score matrix
  * model/BPR.py:76-80 builds, or of any layer whose weights are kept in 8 bits.  The sum is exact in int32 (K <= 131071),
  * then in float32: converted, times sa[m], times sb[n], plus bias[n], each rounded, and rounded once more where c_dtype
- * (TFREC_DT_*) has 16 bits.  C rows are ldc >= N elements apart.  Columns of A and B from K on are not used.  Uses no
- * workspace. */
+ * (TFREC_DT_*) has 16 bits.  C rows are ldc >= N elements apart.  Columns of A and B from K on are not used.  The
+ * values of C may share no byte with an operand, a scale or the bias.  Uses no workspace. */
 int tfrec_matmul_i8(tfrec_ctx *ctx, const int8_t *d_A, int64_t lda, const float *d_sa, int64_t M,
                     const int8_t *d_B, int64_t ldb, const float *d_sb, int64_t N, int64_t K,
                     const float *d_bias, void *d_C, int c_dtype, int64_t ldc);

@@ -33,3 +33,36 @@ def test_a_norm_within_a_tensor_is_refused(lib):
                        (A + 4096 + 68, "null context"), (A + 65536, "tensor 1"), (A + 65536 + 64, "tensor 1"), (A + 65536 + 68, "null context"),
                        (A + 8192, "null context"), (None, "null context")):                       # (the third tensor is empty)
         refused(lib, clip(lib, grads, outs, counts, types, norm), word)
+
+
+def bytes_of(at, pitch, length, n):
+    return {at + r * pitch + i for r in range(n) for i in range(length)}
+
+
+def test_rows_overlap_against_sets_of_bytes(lib):
+    f = lib.tfrec_rows_overlap
+    f.argtypes, f.restype = [C.c_size_t] + [C.c_int64] * 3 + [C.c_size_t] + [C.c_int64] * 3, C.c_int
+    rng = np.random.default_rng(1)
+    verdicts = [0, 0]
+    for _ in range(4000):
+        rows = []
+        for _ in range(2):
+            length, n = int(rng.integers(0, 12)), int(rng.integers(0, 7))
+            rows.append((1000 + int(rng.integers(0, 80)), length + int(rng.integers(0, 20)) or 1, length, n))
+        if rng.random() < 0.3:                        # columns of one matrix
+            rows[1] = (rows[1][0], rows[0][1], min(rows[1][2], rows[0][1]), rows[1][3])
+        want = bool(bytes_of(*rows[0]) & bytes_of(*rows[1]))
+        assert f(*rows[0], *rows[1]) == want == f(*rows[1], *rows[0]), rows
+        verdicts[want] += 1
+    assert min(verdicts) > 500
+
+
+def test_rows_overlap_far_out(lib):
+    """Spans beyond 2^32 bytes, a vector between a matrix's rows, and one that crosses from a gap into a row."""
+    f = lib.tfrec_rows_overlap
+    f.argtypes, f.restype = [C.c_size_t] + [C.c_int64] * 3 + [C.c_size_t] + [C.c_int64] * 3, C.c_int
+    at, pitch, length, n = 1 << 40, 1 << 20, 1000, 1 << 16
+    row = at + 60000 * pitch
+    for lo, size, want in ((row, 4, 1), (row + 999, 4, 1), (row + 1000, pitch - 1000, 0), (row + 1000, pitch - 999, 1), (row - 4, 4, 0), (row - 4, 5, 1),
+                           (at + n * pitch, 4, 0), (at + (n - 1) * pitch + 1000, 4, 0), (at - 4, 4, 0), (at - 4, 5, 1), (at - 4, 1 << 40, 1)):
+        assert f(at, pitch, length, n, lo, size, size, 1) == want == f(lo, size, size, 1, at, pitch, length, n), (lo, size)

@@ -150,6 +150,41 @@ int tfrec_check_i8(const char *name, const int8_t *q, int64_t rows, int64_t ld, 
     return TFREC_OK;
 }
 
+// n rows of len bytes, pitch bytes apart
+struct RowBytes { uintptr_t at; int64_t pitch, len, n; };
+
+// [lo, hi) and any of the rows
+static bool meets(uintptr_t lo, uintptr_t hi, const RowBytes &b)
+{
+    const uintptr_t end = b.at + (b.n - 1) * b.pitch + b.len;
+    if (hi <= b.at || lo >= end) return false;
+    if (lo <= b.at) return true;
+    const int64_t r = (int64_t)(lo - b.at) / b.pitch, off = (int64_t)(lo - b.at) % b.pitch;
+    return off < b.len || b.at + (r + 1) * b.pitch < hi;         // within row r, or the next row (there is one: lo < end) begins before hi
+}
+
+// Any byte in common?  Rows that merely lie between each other's have none.  The spans of two buffers that have nothing to do with
+// each other are apart, which is all that is looked at then.
+static bool rows_overlap(RowBytes a, RowBytes b)
+{
+    if (a.n <= 0 || b.n <= 0 || a.len <= 0 || b.len <= 0) return false;
+    if (a.n > b.n) { const RowBytes t = a; a = b; b = t; }
+    const uintptr_t end_a = a.at + (a.n - 1) * a.pitch + a.len, end_b = b.at + (b.n - 1) * b.pitch + b.len;
+    if (end_a <= b.at || end_b <= a.at) return false;
+    for (int64_t i = 0; i < a.n; ++i)
+        if (meets(a.at + i * a.pitch, a.at + i * a.pitch + a.len, b)) return true;
+    return false;
+}
+
+// the same for callers without the struct (tests)
+extern "C" int tfrec_rows_overlap(uintptr_t at, int64_t pitch, int64_t len, int64_t n, uintptr_t at2, int64_t pitch2, int64_t len2, int64_t n2)
+{
+    return rows_overlap({at, pitch, len, n}, {at2, pitch2, len2, n2});
+}
+
+// a contiguous array as one row (null: none)
+static RowBytes array_bytes(const void *p, int64_t n, int64_t size) { return {(uintptr_t)p, n * size, n * size, p ? 1 : 0}; }
+
 extern "C" int tfrec_quantize_rows_i8(tfrec_ctx *ctx, const void *d_X, int x_dtype, int64_t n_rows, int64_t ldx, int64_t d,
                                       const int32_t *d_rows, int64_t n, int8_t *d_q, int64_t ldq, float *d_scale)
 {
@@ -162,6 +197,11 @@ extern "C" int tfrec_quantize_rows_i8(tfrec_ctx *ctx, const void *d_X, int x_dty
     TF_TRY(tfrec_check_i8("the 8-bit matrix", d_q, n, ldq, d));
     TF_TRY(tfrec_ctx_enter(ctx));
     if (n == 0) return TFREC_OK;
+    const int64_t es = x_dtype == TFREC_DT_F32 ? 4 : 2;
+    const RowBytes q{(uintptr_t)d_q, ldq, up16(d), n}, s = array_bytes(d_scale, n, 4), x{(uintptr_t)d_X, ldx * es, d * es, d_rows ? n_rows : n}, ids = array_bytes(d_rows, n, 4);
+    for (const RowBytes &o : {q, s})
+        TF_REQUIRE(!rows_overlap(o, x) && !rows_overlap(o, ids), TFREC_EINVAL, "an output overlaps the source rows or their list");
+    TF_REQUIRE(!rows_overlap(q, s), TFREC_EINVAL, "the 8-bit rows and the scales overlap");
     return tfrec_quantize_rows(ctx, d_X, x_dtype, n_rows, ldx, d, d_rows, n, d_q, ldq, d_scale);
 }
 
@@ -647,6 +687,10 @@ extern "C" int tfrec_matmul_i8(tfrec_ctx *ctx, const int8_t *d_A, int64_t lda, c
     TF_REQUIRE(((uintptr_t)d_C & (c_dtype == TFREC_DT_F32 ? 3u : 1u)) == 0, TFREC_EINVAL, "C is not aligned to its type");
     TF_TRY(tfrec_ctx_enter(ctx));
     if (M == 0 || N == 0) return TFREC_OK;
+    const int64_t es = c_dtype == TFREC_DT_F32 ? 4 : 2;
+    const RowBytes c{(uintptr_t)d_C, ldc * es, N * es, M};
+    for (const RowBytes &r : {RowBytes{(uintptr_t)d_A, lda, K, M}, RowBytes{(uintptr_t)d_B, ldb, K, N}, array_bytes(d_sa, M, 4), array_bytes(d_sb, N, 4), array_bytes(d_bias, N, 4)})
+        TF_REQUIRE(!rows_overlap(c, r), TFREC_EINVAL, "C overlaps an operand, a scale or the bias");
     const MatmulArgs a{d_A, d_B, d_sa, d_sb, d_bias, d_C, lda, ldb, ldc, M, N, K};
     if (c_dtype == TFREC_DT_BF16) return launch_matmul<__bf16>(ctx, a);
     if (c_dtype == TFREC_DT_F16) return launch_matmul<_Float16>(ctx, a);
