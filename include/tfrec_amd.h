@@ -326,9 +326,10 @@ int tfrec_dns_select(tfrec_ctx *ctx, const float *d_P, const float *d_Q, const f
 /* The gradients of the BPR loss without a step (the loss of tfrec_bpr_sgd_step, model/BPR.py:36-48): d_gP [U,d],
  * d_gQ [I,d] and d_gb [I] are zeroed and receive the summed gradient of every row the batch touches (l2 terms
  * included).  axpy(table, gradient, -lr) on the three tables is then bit for bit tfrec_bpr_sgd_step.  For steps
- * that look at the whole gradient first (tfrec_grad_clip).  The six tables must not overlap.  d_loss as there.  Can be
- * captured into a HIP graph once a call of that size was made (its scratch, the workspace and a sorted index, does not grow
- * under capture: TFREC_ENOMEM); graphs captured from one context share that scratch. */
+ * that look at the whole gradient first (tfrec_grad_clip).  The gradient tables and d_loss (as there) may overlap
+ * nothing else that the call is handed.  Can be captured into a HIP graph once a call of that size was made (its scratch,
+ * the workspace and a sorted index, does not grow under capture: TFREC_ENOMEM); graphs captured from one context share that
+ * scratch. */
 int tfrec_bpr_grads(tfrec_ctx *ctx, const float *d_P, const float *d_Q, const float *d_b, int64_t U, int64_t I, int d,
                     const int32_t *d_users, const int32_t *d_pos, const int32_t *d_neg, int64_t B, float reg,
                     float *d_gP, float *d_gQ, float *d_gb, double *d_loss);

@@ -1307,6 +1307,19 @@ extern "C" int tfrec_bpr_grads(tfrec_ctx *ctx, const float *d_P, const float *d_
             for (int j = i + 1; j < 6; ++j)
                 TF_REQUIRE(!at[j] || (uintptr_t)(at[i] + len[i]) <= (uintptr_t)at[j] || (uintptr_t)(at[j] + len[j]) <= (uintptr_t)at[i], TFREC_EINVAL,
                            j < 3 ? "two gradient tables overlap" : "a gradient table overlaps the parameters");
+        const int32_t *lists[3] = {d_users, d_pos, d_neg};
+        const int64_t nb = B > 0 ? B : 0;
+        for (const int32_t *x : lists)
+            for (int i = 0; i < 3; ++i)
+                TF_REQUIRE(!x || !nb || (uintptr_t)(x + nb) <= (uintptr_t)at[i] || (uintptr_t)(at[i] + len[i]) <= (uintptr_t)x, TFREC_EINVAL,
+                           "a gradient table overlaps the batch");
+        if (d_loss) {
+            const uintptr_t lo = (uintptr_t)d_loss, hi = (uintptr_t)(d_loss + 2);
+            for (int i = 0; i < 6; ++i)
+                TF_REQUIRE(!at[i] || hi <= (uintptr_t)at[i] || (uintptr_t)(at[i] + len[i]) <= lo, TFREC_EINVAL, "the loss overlaps a table");
+            for (const int32_t *x : lists)
+                TF_REQUIRE(!x || !nb || hi <= (uintptr_t)x || (uintptr_t)(x + nb) <= lo, TFREC_EINVAL, "the loss overlaps the batch");
+        }
     }
     TF_TRY(tfrec_ctx_enter(ctx));
     TF_TRY(check_step_args(d_P, d_Q, d_b, U, I, d, d_users, d_pos, d_neg, B));

@@ -540,6 +540,12 @@ class Device:
         B = _shape(users)[0]
         if _shape(gP) != (U, d) or _shape(gQ) != (I, d) or _shape(gb) != (I,):
             raise ValueError("gradients need the shapes of their tables")
+        if _shape(Q) != (I, d) or _numel(b) != I or _numel(pos) < B or _numel(neg) < B or (loss is not None and _numel(loss) < 2):
+            raise ValueError("need Q [I, d], b [I], three index arrays of one length and a loss of two values")
+        for x, want in ((P, "float32"), (Q, "float32"), (b, "float32"), (gP, "float32"), (gQ, "float32"), (gb, "float32"),
+                        (users, "int32"), (pos, "int32"), (neg, "int32"), (loss, "float64")):
+            if x is not None and (_dtype_name(x) != want or _gpu_of(x) != self.device):
+                raise ValueError("tables and gradients have to be float32, indices int32, the loss float64, all on GPU %d" % self.device)
         _lib.check(self.lib.tfrec_bpr_grads(self.h, _ptr(P), _ptr(Q), _ptr(b), U, I, d, _ptr(users), _ptr(pos), _ptr(neg), B, float(reg),
                                             _ptr(gP), _ptr(gQ), _ptr(gb), _ptr(loss)))
 
