@@ -116,10 +116,12 @@ static int launch_quantize(tfrec_ctx *ctx, const void *X, int64_t n_rows, int64_
 {
     auto go = [&]<int LPR, int CH>() -> int {
         constexpr int GPB = 256 / LPR;
-        const int64_t blocks = (n + GPB - 1) / GPB;
-        TF_REQUIRE(blocks < (1ll << 31), TFREC_EUNSUP, "too many rows");
-        quantize_rows_kernel<T, LPR, CH><<<(unsigned)blocks, 256, 0, ctx->stream>>>((const T *)X, n_rows, ldx, d, rows, n, q, ldq, scale, ctx->d_flags);
-        TF_HIP(hipGetLastError());
+        for (int64_t r = 0; r < n; r += TF_LAUNCH_ROWS * GPB) {
+            const int64_t m = n - r < TF_LAUNCH_ROWS * GPB ? n - r : TF_LAUNCH_ROWS * GPB;
+            quantize_rows_kernel<T, LPR, CH><<<(unsigned)((m + GPB - 1) / GPB), 256, 0, ctx->stream>>>(
+                (const T *)X + (rows ? 0 : r * ldx), n_rows, ldx, d, rows ? rows + r : nullptr, m, q + r * ldq, ldq, scale + r, ctx->d_flags);
+            TF_HIP(hipGetLastError());
+        }
         return TFREC_OK;
     };
     const int64_t chunks = (d + 15) / 16;
@@ -624,7 +626,7 @@ static int launch_big(tfrec_ctx *ctx, const MatmulArgs &a)
 {
     using G = BigGeom<WM, WN, FM, FN, NB>;
     const int64_t tm = (a.M + G::SIDE - 1) / G::SIDE, tn = (a.N + G::SIDE - 1) / G::SIDE, tiles = tm * tn;
-    TF_REQUIRE(tiles < (1ll << 28), TFREC_EUNSUP, "the product is too large for one launch");
+    TF_TRY(check_launch((tiles + 7) / 8 * 8, 64 * G::NW));
     static std::atomic<uint64_t> done{0};
     TF_TRY(tfrec_raise_lds_limit(ctx, reinterpret_cast<const void *>(&matmul_i8_big_kernel<T, WM, WN, FM, FN, NB>), G::LDS, done));
     matmul_i8_big_kernel<T, WM, WN, FM, FN, NB><<<(unsigned)((tiles + 7) / 8 * 8), 64 * G::NW, G::LDS, ctx->stream>>>(a, (int)tm, (int)tn);
@@ -654,11 +656,11 @@ static int launch_matmul(tfrec_ctx *ctx, const MatmulArgs &a)
     if (near && !stores && a.M > 128 && a.K >= 512 && big >= 160) return launch_big<T, 2, 4, 4, 2, 2>(ctx, a);
     if (near && !stores && a.K >= 256 && rows_us > tiles_us) return mid <= 256 ? launch_big<T, 2, 2, 2, 2, 4>(ctx, a) : launch_big<T, 2, 2, 2, 2, 2>(ctx, a);
     if (stores || (a.M > 64 && mid >= 192)) {
-        TF_REQUIRE(mid < (1ll << 31), TFREC_EUNSUP, "the product is too large for one launch");
+        TF_TRY(check_launch(mid, 256));
         matmul_i8_kernel<T><<<(unsigned)mid, 256, 0, ctx->stream>>>(a);
     } else {
         const int64_t nb = (a.N + 15) / 16;
-        TF_REQUIRE(nb < (1ll << 31), TFREC_EUNSUP, "the product is too large for one launch");
+        TF_TRY(check_launch(nb, 64 * 8));
         auto go = [&]<int MT, int KW>() { matmul_i8_rows_kernel<T, MT, KW><<<dim3((unsigned)nb, (unsigned)((a.M + 16 * MT - 1) / (16 * MT))), 64 * KW, 0, ctx->stream>>>(a); };
         auto waves = [&]<int MT>() {
             if (a.K <= 256) go.template operator()<MT, 1>();
@@ -691,8 +693,15 @@ extern "C" int tfrec_matmul_i8(tfrec_ctx *ctx, const int8_t *d_A, int64_t lda, c
     const RowBytes c{(uintptr_t)d_C, ldc * es, N * es, M};
     for (const RowBytes &r : {RowBytes{(uintptr_t)d_A, lda, K, M}, RowBytes{(uintptr_t)d_B, ldb, K, N}, array_bytes(d_sa, M, 4), array_bytes(d_sb, N, 4), array_bytes(d_bias, N, 4)})
         TF_REQUIRE(!rows_overlap(c, r), TFREC_EINVAL, "C overlaps an operand, a scale or the bias");
-    const MatmulArgs a{d_A, d_B, d_sa, d_sb, d_bias, d_C, lda, ldb, ldc, M, N, K};
-    if (c_dtype == TFREC_DT_BF16) return launch_matmul<__bf16>(ctx, a);
-    if (c_dtype == TFREC_DT_F16) return launch_matmul<_Float16>(ctx, a);
-    return launch_matmul<float>(ctx, a);
+    // (pieces of 2^26 rows of A and of B; the sums are integers: no result depends on it)
+    constexpr int64_t PIECE = 16 * TF_LAUNCH_ROWS;
+    for (int64_t m = 0; m < M; m += PIECE)
+        for (int64_t n = 0; n < N; n += PIECE) {
+            const MatmulArgs a{d_A + m * lda, d_B + n * ldb, d_sa + m, d_sb + n, d_bias ? d_bias + n : nullptr, (char *)d_C + (m * ldc + n) * es, lda, ldb, ldc,
+                               M - m < PIECE ? M - m : PIECE, N - n < PIECE ? N - n : PIECE, K};
+            if (c_dtype == TFREC_DT_BF16) TF_TRY(launch_matmul<__bf16>(ctx, a));
+            else if (c_dtype == TFREC_DT_F16) TF_TRY(launch_matmul<_Float16>(ctx, a));
+            else TF_TRY(launch_matmul<float>(ctx, a));
+        }
+    return TFREC_OK;
 }

@@ -735,8 +735,7 @@ __global__ __launch_bounds__(256) void score_small_i8_kernel(ScoreI8Args a)
 
 __global__ __launch_bounds__(256) void no_entries_kernel(int32_t *__restrict__ ids, float *__restrict__ scores, int64_t n)
 {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i < n) { ids[i] = -1; scores[i] = -INFINITY; }
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) { ids[i] = -1; scores[i] = -INFINITY; }
 }
 
 // ------------------------------------------------------------------------------------------
@@ -791,7 +790,7 @@ static int by_row_lanes(int d, F &&f)
 static int launch_max(tfrec_ctx *ctx, const MaxArgs &m)
 {
     const int64_t grid = (int64_t)((m.splits + 7) / 8) * 8 * ((m.user_groups + 3) / 4);
-    TF_REQUIRE(grid < (1ll << 31), TFREC_EUNSUP, "too many users and items for one launch");
+    TF_TRY(check_launch(grid, 256));
     auto go = [&]<int KS, int UW>() -> int {
         score_max_i8_kernel<KS, UW><<<(unsigned)grid, 256, 0, ctx->stream>>>(m);
         TF_HIP(hipGetLastError());
@@ -832,16 +831,30 @@ int tfrec_score_i8(tfrec_ctx *ctx, ScoreI8Args a)
 {
     if (a.n == 0) return TFREC_OK;
     if (a.n_items == 0) {
-        no_entries_kernel<<<(unsigned)((a.n * a.k + 255) / 256), 256, 0, ctx->stream>>>(a.out_ids, a.out_scores, a.n * a.k);
+        const int64_t blocks = (a.n * a.k + 255) / 256;
+        no_entries_kernel<<<(unsigned)(blocks < TF_LAUNCH_ROWS ? blocks : TF_LAUNCH_ROWS), 256, 0, ctx->stream>>>(a.out_ids, a.out_scores, a.n * a.k);
         TF_HIP(hipGetLastError());
         return TFREC_OK;
     }
     a.flags = ctx->d_flags;
+    // users u0 .. u0 + n of the call
+    auto listed = [&](int64_t u0, int64_t n) {
+        ScoreI8Args s = a;
+        s.n = n;
+        s.users = a.users + u0;
+        if (a.p_compact) { s.Pq = a.Pq + u0 * a.ldp; s.sp = a.sp + u0; }
+        s.out_ids = a.out_ids + u0 * a.k;
+        s.out_scores = a.out_scores + u0 * a.k;
+        return s;
+    };
     if (a.n_items <= SMALL_ITEMS)
         return by_row_lanes(a.d, [&]<int LPI>() -> int {
-            if (list_for(a.k) == 512) score_small_i8_kernel<LPI, 512><<<(unsigned)a.n, 256, 0, ctx->stream>>>(a);
-            else score_small_i8_kernel<LPI, 1024><<<(unsigned)a.n, 256, 0, ctx->stream>>>(a);
-            TF_HIP(hipGetLastError());
+            for (int64_t u0 = 0; u0 < a.n; u0 += TF_LAUNCH_ROWS) {
+                const ScoreI8Args s = listed(u0, a.n - u0 < TF_LAUNCH_ROWS ? a.n - u0 : TF_LAUNCH_ROWS);
+                if (list_for(a.k) == 512) score_small_i8_kernel<LPI, 512><<<(unsigned)s.n, 256, 0, ctx->stream>>>(s);
+                else score_small_i8_kernel<LPI, 1024><<<(unsigned)s.n, 256, 0, ctx->stream>>>(s);
+                TF_HIP(hipGetLastError());
+            }
             return TFREC_OK;
         });
     MaxArgs m{};
@@ -855,12 +868,7 @@ int tfrec_score_i8(tfrec_ctx *ctx, ScoreI8Args a)
     m.slack = (float *)tfrec_ws_take(ctx, slack);
     TF_REQUIRE(m.bound != nullptr && m.group_bound != nullptr && m.slack != nullptr, TFREC_ENOMEM, "internal: workspace carve failed");
     for (int64_t u0 = 0; u0 < a.n; u0 += per_pass) {
-        m.s = a;
-        m.s.n = a.n - u0 < per_pass ? a.n - u0 : per_pass;
-        m.s.users = a.users + u0;
-        if (a.p_compact) { m.s.Pq = a.Pq + u0 * a.ldp; m.s.sp = a.sp + u0; }
-        m.s.out_ids = a.out_ids + u0 * a.k;
-        m.s.out_scores = a.out_scores + u0 * a.k;
+        m.s = listed(u0, a.n - u0 < per_pass ? a.n - u0 : per_pass);
         m.splits = split_items(m.s.n, m.groups, a.d, &m.groups_per_split);
         const int users = 32 * sets_per_wave(m.s.n, a.d);
         m.user_groups = (int)((m.s.n + users - 1) / users);

@@ -26,6 +26,14 @@ struct ScoreI8Args {
     uint32_t *flags;
 };
 
+// A launch has to stay below 2^32 threads.  What has a workgroup per row, user or 16 columns is launched in pieces of this many.
+static constexpr int64_t TF_LAUNCH_ROWS = 1ll << 22;
+static inline int check_launch(int64_t blocks, int threads)
+{
+    TF_REQUIRE(blocks * threads < (1ll << 32), TFREC_EUNSUP, "%lld workgroups of %d threads are too many for one launch", (long long)blocks, threads);
+    return TFREC_OK;
+}
+
 // raises a kernel's dynamic-LDS limit once per device (eval.hip)
 int tfrec_raise_lds_limit(tfrec_ctx *ctx, const void *kernel, int bytes, std::atomic<uint64_t> &done);
 // the layout every 8-bit matrix has to have (quant.hip)
