@@ -380,6 +380,15 @@ int tfrec_matmul_i8(tfrec_ctx *ctx, const int8_t *d_A, int64_t lda, const float 
                     const int8_t *d_B, int64_t ldb, const float *d_sb, int64_t N, int64_t K,
                     const float *d_bias, void *d_C, int c_dtype, int64_t ldc);
 
+/* Which of its kernels tfrec_matmul_i8 runs for a product of these sizes (up to 2^26 rows of either operand; what is larger is
+ * cut into such pieces): for programs that profile it, and for tests of each kernel.  The results do not depend on it. */
+#define TFREC_I8_ROWS 0             /* 16 rows of B against all rows of A */
+#define TFREC_I8_SHORT 1            /* 128 x 128 tiles of short rows */
+#define TFREC_I8_TILES_256 2        /* 256 x 256 tiles */
+#define TFREC_I8_TILES_128 3        /* 128 x 128 tiles in two buffers, two workgroups a CU */
+#define TFREC_I8_TILES_128_DEEP 4   /* 128 x 128 tiles in four buffers, one workgroup a CU */
+int tfrec_matmul_i8_kernel(int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb, int c_dtype);
+
 /* ---- evaluation ---------------------------------------------------------------------------- */
 #define TFREC_SCORE_F32 0    /* exact float32: score = fma chain over f ascending, starting at b[i] */
 #define TFREC_SCORE_BF16 1   /* operands rounded to bfloat16, float32 accumulation (MFMA)            */

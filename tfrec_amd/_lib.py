@@ -15,6 +15,7 @@ LIB_PATH = os.environ.get("TFREC_AMD_LIB") or os.path.join(_HERE, "lib", "libtfr
 OK, EINVAL, EHIP, ENOMEM, EINDEX, EUNSUP = 0, -1, -2, -3, -4, -5
 SCORE_F32, SCORE_BF16, SCORE_I8 = 0, 1, 2
 DT_F32, DT_BF16, DT_F16 = 0, 1, 2
+I8_ROWS, I8_SHORT, I8_TILES_256, I8_TILES_128, I8_TILES_128_DEEP = range(5)
 
 _p = C.c_void_p
 _i64 = C.c_int64
@@ -80,6 +81,7 @@ SIGNATURES = {
     "tfrec_grads_clip": (_int, [_p, _p, _d, _p]),
     "tfrec_quantize_rows_i8": (_int, [_p, _p, _int, _i64, _i64, _i64, _p, _i64, _p, _i64, _p]),
     "tfrec_matmul_i8": (_int, [_p, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _i64, _p, _p, _int, _i64]),
+    "tfrec_matmul_i8_kernel": (_int, [_i64, _i64, _i64, _i64, _i64, _int]),
     "tfrec_score_topk_i8": (_int, [_p, _p, _i64, _p, _i64, _int, _p, _i64, _p, _p, _i64, _int, _i64, _i64, _p, _i64, _p, _p, _int, _p, _p]),
     "tfrec_axpy": (_int, [_p, _p, _p, _f, _i64]),
     "tfrec_apr_adagrad_step": (_int, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _int, _p, _p, _p, _i64,

@@ -645,20 +645,32 @@ static int launch_big(tfrec_ctx *ctx, const MatmulArgs &a)
 //     LDS and several workgroups a CU serves best: 2048 x 200000 x 64 in float32 300 (5.5 TB/s; a fill of C alone 240) against
 //     454, 2048 x 50000 x 256 in float32 113 / 151, in bfloat16 even, x 512 even / in bfloat16 128 / 100;
 //   16 rows of B at a time for everything else: small products get workgroups enough, few rows of A are bound by reading B.
+static int choose_matmul(int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb, int c_bytes)
+{
+    const int64_t big = ((M + 255) / 256) * ((N + 255) / 256), mid = ((M + 127) / 128) * ((N + 127) / 128);
+    const bool near = lda < (1 << 24) && ldb < (1 << 24);        // a tile's rows are within 4 GB of its first
+    const double rows_us = (double)N * (double)K * (1.6e-7 + 6.2e-9 * (double)M);
+    const double tiles_us = (2.2 + 3.65e-3 * (double)K) * (mid > 256 ? (double)mid / 230. : 1.);
+    const bool stores = M > 64 && mid >= 192 && K <= 128 * (int64_t)c_bytes;
+    if (near && !stores && M > 128 && K >= 512 && big >= 160) return TFREC_I8_TILES_256;
+    if (near && !stores && K >= 256 && rows_us > tiles_us) return mid <= 256 ? TFREC_I8_TILES_128_DEEP : TFREC_I8_TILES_128;
+    return stores || (M > 64 && mid >= 192) ? TFREC_I8_SHORT : TFREC_I8_ROWS;
+}
+
 template <class T>
 static int launch_matmul(tfrec_ctx *ctx, const MatmulArgs &a)
 {
-    const int64_t big = ((a.M + 255) / 256) * ((a.N + 255) / 256), mid = ((a.M + 127) / 128) * ((a.N + 127) / 128);
-    const bool near = a.lda < (1 << 24) && a.ldb < (1 << 24);        // a tile's rows are within 4 GB of its first
-    const double rows_us = (double)a.N * (double)a.K * (1.6e-7 + 6.2e-9 * (double)a.M);
-    const double tiles_us = (2.2 + 3.65e-3 * (double)a.K) * (mid > 256 ? (double)mid / 230. : 1.);
-    const bool stores = a.M > 64 && mid >= 192 && a.K <= 128 * (int64_t)sizeof(T);
-    if (near && !stores && a.M > 128 && a.K >= 512 && big >= 160) return launch_big<T, 2, 4, 4, 2, 2>(ctx, a);
-    if (near && !stores && a.K >= 256 && rows_us > tiles_us) return mid <= 256 ? launch_big<T, 2, 2, 2, 2, 4>(ctx, a) : launch_big<T, 2, 2, 2, 2, 2>(ctx, a);
-    if (stores || (a.M > 64 && mid >= 192)) {
-        TF_TRY(check_launch(mid, 256));
-        matmul_i8_kernel<T><<<(unsigned)mid, 256, 0, ctx->stream>>>(a);
-    } else {
+    switch (choose_matmul(a.M, a.N, a.K, a.lda, a.ldb, sizeof(T))) {
+    case TFREC_I8_TILES_256: return launch_big<T, 2, 4, 4, 2, 2>(ctx, a);
+    case TFREC_I8_TILES_128_DEEP: return launch_big<T, 2, 2, 2, 2, 4>(ctx, a);
+    case TFREC_I8_TILES_128: return launch_big<T, 2, 2, 2, 2, 2>(ctx, a);
+    case TFREC_I8_SHORT: {
+        const int64_t tiles = ((a.M + 127) / 128) * ((a.N + 127) / 128);
+        TF_TRY(check_launch(tiles, 256));
+        matmul_i8_kernel<T><<<(unsigned)tiles, 256, 0, ctx->stream>>>(a);
+        break;
+    }
+    default: {
         const int64_t nb = (a.N + 15) / 16;
         TF_TRY(check_launch(nb, 64 * 8));
         auto go = [&]<int MT, int KW>() { matmul_i8_rows_kernel<T, MT, KW><<<dim3((unsigned)nb, (unsigned)((a.M + 16 * MT - 1) / (16 * MT))), 64 * KW, 0, ctx->stream>>>(a); };
@@ -672,8 +684,14 @@ static int launch_matmul(tfrec_ctx *ctx, const MatmulArgs &a)
         else if (a.M <= 64) waves.template operator()<4>();
         else waves.template operator()<8>();
     }
+    }
     TF_HIP(hipGetLastError());
     return TFREC_OK;
+}
+
+extern "C" int tfrec_matmul_i8_kernel(int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb, int c_dtype)
+{
+    return choose_matmul(M, N, K, lda, ldb, c_dtype == TFREC_DT_F32 ? 4 : 2);
 }
 
 extern "C" int tfrec_matmul_i8(tfrec_ctx *ctx, const int8_t *d_A, int64_t lda, const float *d_sa, int64_t M, const int8_t *d_B, int64_t ldb,
