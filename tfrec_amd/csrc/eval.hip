@@ -1065,7 +1065,8 @@ static int launch_score_cap(tfrec_ctx *ctx, const ScoreArgs &a, int D, int mode,
     return TFREC_EUNSUP;
 }
 
-int tfrec_merge_lists(tfrec_ctx *ctx, const int32_t *ids, const float *scores, int G, int64_t n, int k, int32_t *out_ids,
+// G lists of k per user -> the k best of them (G * k <= 2048)
+static int merge_lists(tfrec_ctx *ctx, const int32_t *ids, const float *scores, int G, int64_t n, int k, int32_t *out_ids,
                        float *out_scores)
 {
     const int blocks = (int)((n + 3) / 4);
@@ -1086,7 +1087,7 @@ extern "C" int tfrec_topk_merge(tfrec_ctx *ctx, const int32_t *d_ids, const floa
     TF_REQUIRE(G >= 1 && n >= 0 && k >= 1, TFREC_EINVAL, "bad merge shape G=%d n=%lld k=%d", G, (long long)n, k);
     if (n == 0) return TFREC_OK;
     TF_REQUIRE(d_ids && d_scores && d_out_ids && d_out_scores, TFREC_EINVAL, "null pointer");
-    return tfrec_merge_lists(ctx, d_ids, d_scores, G, n, k, d_out_ids, d_out_scores);
+    return merge_lists(ctx, d_ids, d_scores, G, n, k, d_out_ids, d_out_scores);
 }
 
 static int pad_dim(int d, int mode)
@@ -1154,9 +1155,9 @@ static int plan_score(const float *d_Q, int d, int64_t item_lo, int64_t item_hi,
 
 // TFREC_SCORE_I8: the listed users' rows and the item rows are quantised into the workspace, then scored there
 static size_t quantized_bytes(int64_t rows, int d) { return tf_align((size_t)rows * tf_align(d, 16)) + tf_align((size_t)rows * 4); }
-static size_t score_i8_need(int64_t n, int64_t n_items, int d, int k)
+static size_t score_i8_need(int64_t n, int64_t n_items, int d)
 {
-    return quantized_bytes(n, d) + quantized_bytes(n_items, d) + tfrec_score_i8_bytes(n, n_items, d, k) + 1024;
+    return quantized_bytes(n, d) + quantized_bytes(n_items, d) + tfrec_score_i8_bytes(n, n_items) + 1024;
 }
 
 static int score_topk_quantized(tfrec_ctx *ctx, const float *d_P, const float *d_Q, const float *d_b, int d, int64_t item_lo, int64_t item_hi,
@@ -1166,7 +1167,7 @@ static int score_topk_quantized(tfrec_ctx *ctx, const float *d_P, const float *d
     TF_REQUIRE(cap_for_k(k) != 0, TFREC_EUNSUP, "top-k above 240 is not supported (k=%d)", k);
     TF_REQUIRE(d >= 1 && d <= 256, TFREC_EUNSUP, "factor size d=%d is not supported for this score mode", d);
     const int64_t n_items = item_hi - item_lo, ld = (int64_t)tf_align(d, 16);
-    TF_TRY(tfrec_ws_require(ctx, ctx->ws_used + score_i8_need(n, n_items, d, k)));
+    TF_TRY(tfrec_ws_require(ctx, ctx->ws_used + score_i8_need(n, n_items, d)));
     int8_t *pq = (int8_t *)tfrec_ws_take(ctx, (size_t)n * ld), *qq = (int8_t *)tfrec_ws_take(ctx, (size_t)n_items * ld);
     float *sp = (float *)tfrec_ws_take(ctx, (size_t)n * 4), *sq = (float *)tfrec_ws_take(ctx, (size_t)n_items * 4);
     TF_REQUIRE(pq && qq && sp && sq, TFREC_ENOMEM, "internal: workspace carve failed");
@@ -1257,16 +1258,16 @@ static int score_topk_impl(tfrec_ctx *ctx, const float *d_P, const float *d_Q, c
 #endif
         else TF_TRY(launch_score_cap<512>(ctx, a, D, score_mode, user_blocks, splits));
         if (splits > 1 && !pl.part2_bytes) {
-            TF_TRY(tfrec_merge_lists(ctx, part_ids, part_sc, splits, nn, k, d_out_ids + (size_t)u0 * k, d_out_scores + (size_t)u0 * k));
+            TF_TRY(merge_lists(ctx, part_ids, part_sc, splits, nn, k, d_out_ids + (size_t)u0 * k, d_out_scores + (size_t)u0 * k));
         } else if (splits > 1) {
             // two levels: groups of lists first (the total order makes the merge of merged lists the merge of all)
             const int g1 = merge_group(k), groups = (splits + g1 - 1) / g1;
             for (int g = 0; g < groups; ++g) {
                 const int cnt = splits - g * g1 < g1 ? splits - g * g1 : g1;
                 const size_t src = (size_t)g * g1 * nn * k, dst = (size_t)g * nn * k;
-                TF_TRY(tfrec_merge_lists(ctx, part_ids + src, part_sc + src, cnt, nn, k, part2_ids + dst, part2_sc + dst));
+                TF_TRY(merge_lists(ctx, part_ids + src, part_sc + src, cnt, nn, k, part2_ids + dst, part2_sc + dst));
             }
-            TF_TRY(tfrec_merge_lists(ctx, part2_ids, part2_sc, groups, nn, k, d_out_ids + (size_t)u0 * k, d_out_scores + (size_t)u0 * k));
+            TF_TRY(merge_lists(ctx, part2_ids, part2_sc, groups, nn, k, d_out_ids + (size_t)u0 * k, d_out_scores + (size_t)u0 * k));
         }
     }
     return TFREC_OK;
@@ -1467,7 +1468,7 @@ size_t tfrec_eval_scratch_bytes(int64_t n, int k)
 size_t tfrec_eval_need_bytes(const float *d_Q, int64_t I, int d, int64_t n, int k, int score_mode, int mean_mode)
 {
     const size_t lists = 2 * tf_align(4 * (size_t)n * k) + metrics_host_need(n, k, mean_mode, false) + 4096;
-    if (score_mode == TFREC_SCORE_I8) return cap_for_k(k) && d >= 1 && d <= 256 ? lists + score_i8_need(n, I, d, k) : 0;
+    if (score_mode == TFREC_SCORE_I8) return cap_for_k(k) && d >= 1 && d <= 256 ? lists + score_i8_need(n, I, d) : 0;
     ScorePlan pl;
     if (plan_score(d_Q, d, 0, I, n, k, score_mode, &pl) != TFREC_OK) return 0;
     return lists + pl.total;

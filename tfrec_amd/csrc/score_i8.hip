@@ -763,17 +763,17 @@ static int split_items(int64_t n, int64_t groups, int d, int64_t *groups_per_spl
     return (int)((groups + *groups_per_split - 1) / *groups_per_split);
 }
 
-static size_t slack_bytes(int64_t n, int64_t groups, int d)
+static size_t slack_bytes(int64_t n)
 {
     // (a later, shorter pass has fewer user groups and so up to 2048 splits for its users)
     return tf_align((size_t)4 * (n + 2048 * 32 * 4));
 }
 
-size_t tfrec_score_i8_bytes(int64_t n, int64_t n_items, int d, int k)
+size_t tfrec_score_i8_bytes(int64_t n, int64_t n_items)
 {
     if (n <= 0 || n_items <= SMALL_ITEMS) return 0;
     const int64_t groups = (n_items + 8 * BLOCK - 1) / (8 * BLOCK), per_pass = users_per_pass(n, groups);
-    return tf_align((size_t)per_pass * groups * 64) + tf_align((size_t)per_pass * groups * 4) + slack_bytes(per_pass, groups, d) + 1024;
+    return tf_align((size_t)per_pass * groups * 64) + tf_align((size_t)per_pass * groups * 4) + slack_bytes(per_pass) + 1024;
 }
 
 // calls f.operator()<LPI>() with the lanes an item's row takes
@@ -861,10 +861,10 @@ int tfrec_score_i8(tfrec_ctx *ctx, ScoreI8Args a)
     m.groups = (a.n_items + 8 * BLOCK - 1) / (8 * BLOCK);
     m.pitch = m.groups * 16;
     const int64_t per_pass = users_per_pass(a.n, m.groups);
-    TF_TRY(tfrec_ws_require(ctx, ctx->ws_used + tfrec_score_i8_bytes(a.n, a.n_items, a.d, a.k)));
+    TF_TRY(tfrec_ws_require(ctx, ctx->ws_used + tfrec_score_i8_bytes(a.n, a.n_items)));
     m.bound = (float *)tfrec_ws_take(ctx, (size_t)per_pass * m.pitch * 4);
     m.group_bound = (float *)tfrec_ws_take(ctx, (size_t)per_pass * m.groups * 4);
-    const size_t slack = slack_bytes(per_pass, m.groups, a.d);
+    const size_t slack = slack_bytes(per_pass);
     m.slack = (float *)tfrec_ws_take(ctx, slack);
     TF_REQUIRE(m.bound != nullptr && m.group_bound != nullptr && m.slack != nullptr, TFREC_ENOMEM, "internal: workspace carve failed");
     for (int64_t u0 = 0; u0 < a.n; u0 += per_pass) {

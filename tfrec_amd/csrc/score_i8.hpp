@@ -43,4 +43,4 @@ int tfrec_quantize_rows(tfrec_ctx *ctx, const void *d_X, int x_dtype, int64_t n_
                         int8_t *d_q, int64_t ldq, float *d_scale);
 // Scores and ranks; scratch from the workspace above what is in use (score_i8.hip).
 int tfrec_score_i8(tfrec_ctx *ctx, ScoreI8Args a);
-size_t tfrec_score_i8_bytes(int64_t n, int64_t n_items, int d, int k);        // its scratch
+size_t tfrec_score_i8_bytes(int64_t n, int64_t n_items);        // its scratch

@@ -3,9 +3,6 @@
 #pragma once
 #include "common.hpp"
 
-// G lists of k per user -> the k best of them (eval.hip; G * k <= 2048)
-int tfrec_merge_lists(tfrec_ctx *ctx, const int32_t *ids, const float *scores, int G, int64_t n, int k, int32_t *out_ids, float *out_scores);
-
 // cycle counts of developer builds (the including file may define them first)
 #ifndef TF_PROF_T
 #define TF_PROF_T() 0ull
