@@ -144,8 +144,9 @@ __device__ __forceinline__ double block_sum(double v)
     return v;
 }
 
-// 308 MB of float32 in 3 tensors: 77 us, 4.0 TB/s, what a plain sum of them reads; 40 MB of bfloat16 in 600 tensors 16 us
-// (both from the caches in part).  2048 workgroups: 4096 take 14 us and their norm 1 us more, 1024 take 21 us.
+// 308 MB of float32 in 3 tensors: 77 us, 4.0 TB/s, as much as a plain sum of them reads and two thirds of what grad_scale_kernel
+// moves: a workgroup has one chunk on its way at a time.  40 MB of bfloat16 in 600 tensors 16 us.  2048 workgroups: 4096 take 14 us
+// and their norm 1 us more, 1024 take 21 us.
 // partial sum of workgroup b over its chunks b, b + grid, ...; `first`: the first launch of a call, which sets the partials
 template <class Table>
 __global__ __launch_bounds__(256) void grad_squares_kernel(Table t, double *__restrict__ part, int first)
@@ -173,7 +174,8 @@ __global__ __launch_bounds__(256) void grad_norm_kernel(const double *__restrict
     if (threadIdx.x == 0) *norm = (float)nm;
 }
 
-// 308 MB of float32: 102 us, 6.0 TB/s of reads and writes; 40 MB of bfloat16 in 600 tensors 22 us.
+// 308 MB of float32: 102 us, 6.0 TB/s of reads and writes; 40 MB of bfloat16 in 600 tensors 22 us, of which every workgroup spends
+// some adding the partial sums before it requests its first chunk.
 template <class Table>
 __global__ __launch_bounds__(256) void grad_scale_kernel(Table t, const double *__restrict__ part, int n_part, double max_norm, float *__restrict__ norm)
 {

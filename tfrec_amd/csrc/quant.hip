@@ -15,7 +15,8 @@ static inline bool dtype_ok(int t) { return t == TFREC_DT_F32 || t == TFREC_DT_B
 // ------------------------------------------------------------------------------------------
 // The nearest integer to x / s, ties to even, exactly: r = rint(x * RN(1/s)) is off by at most one, and the remainder
 // x - r s is exact in float32 (both are multiples of ulp(s) where |x| >= s, and |x - r s| < s otherwise), so comparing it
-// with s / 2 decides.  Scales near the subnormal range are lifted by 2^64 first (exact; |x| <= 127.5 s).
+// with s / 2 decides.  Scales near the subnormal range are lifted by 2^64 first (exact; |x| <= 127.5 s, or up to 190 s where s was
+// rounded to one of the smallest subnormal numbers: such a value ends at 127).
 __device__ __forceinline__ int quantize_one(float x, float s, float inv)
 {
     float r = rintf(x * inv);
@@ -33,7 +34,8 @@ struct __attribute__((packed, aligned(sizeof(T)))) Values16 { T v[16]; };
 // LPR threads hold one row (a power of two up to 64: lanes of a wave; 256: the workgroup), CH runs of 16 columns each in
 // registers: one read of the row, one write of a quarter (half) as much.  CH = 0: rows too long for that are read twice,
 // the second time from the caches.
-// Bound by memory: 4096 x 8192 bf16 (96 MB in all) takes 30 us, 3.2 TB/s.
+// Bound by its vector instructions, 30 a value (the vector pipes are busy at least 70 % of the cycles), with nothing of the next row on its
+// way meanwhile: 4096 x 8192 in bfloat16 (100 MB in all) 28 us, 3.6 TB/s; in float32 (168 MB) 29 us.
 template <class T, int LPR, int CH>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(const T *__restrict__ X, int64_t n_rows, int64_t ldx, int64_t d,
                                                             const int32_t *__restrict__ rows, int64_t n, int8_t *__restrict__ q, int64_t ldq,
@@ -435,8 +437,10 @@ __global__ __launch_bounds__(256) void matmul_i8_kernel(MatmulArgs a)
 }
 
 // ---- large products: WM x WN waves, FM x FN blocks of 32 x 32 of C per wave ----------------------------------------------
-// 256 x 256 of C per workgroup (2 x 4 waves of 4 x 2 blocks, two waves a SIMD), bound by the matrix cores (8192 x 8192 x 8192
-// 482 us, 2.28 * 10^15 operations/s), or 128 x 128 (2 x 2 waves of 2 x 2 blocks) where the larger tiles are too few for the chip.
+// 256 x 256 of C per workgroup (2 x 4 waves of 4 x 2 blocks, two waves a SIMD; 8192 x 8192 x 8192 482 us, 2.28 * 10^15
+// operations/s), or 128 x 128 (2 x 2 waves of 2 x 2 blocks) where the larger tiles are too few for the chip.  At 4096 x 8192 x 8192
+// the matrix pipes are busy 55 % of the cycles, at 1.9 GHz, the clock the chip holds under this load; LDS bank conflicts take 21 %
+// of the cycles, the rest are waits between fragments and products.
 // A step takes 128 columns: 4 FM FN matrix instructions a wave.  Rows go from memory straight into LDS
 // (global_load_lds_dwordx4: one kilobyte, eight rows, per instruction and wave), NB buffers: the loads of step s + NB - 1 are
 // issued among the products of step s.  The LDS image has no row padding; position c of row r holds the row's chunk c ^ (r & 7),

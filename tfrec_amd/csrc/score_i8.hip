@@ -24,7 +24,10 @@ typedef int32_t i32x16 __attribute__((ext_vector_type(16)));
 struct __attribute__((packed, aligned(4))) Float4 { float v[4]; };       // 16 bytes at the alignment of a float
 
 static constexpr int BLOCK = 32, CELL = 16;    // items per block (a matrix instruction's rows) and per cell
-static constexpr int SMALL_ITEMS = 4096;       // (16 scores per thread of score_small_i8_kernel)
+// Up to this many items (16 scores per thread) one launch does it, score_small_i8_kernel.  Against the two steps, us: one user x
+// 1682 items x 20 columns 8 / 17, 943 users x 1682 x 20 13 / 23, 943 x 4000 x 128 32 / 33, 6000 x 1000 x 64 51 / 84, 20000 x 1682 x 20
+// 140 / 211; even where many users meet the most items: 6000 x 3700 x 64 86 / 86, 20000 x 4000 x 64 260 / 256, 4096 x 4096 x 128 97 / 89.
+static constexpr int SMALL_ITEMS = 4096;
 static constexpr uint32_t KEY_NONE = 0x007fffffu;      // orderable form of -inf: nothing below or at it is listed
 
 // row of the user table that listed user r reads, and the user's id (the row of the train CSR)
@@ -101,8 +104,8 @@ static constexpr float NO_SCORE = LOWEST * (1.f - 0x1p-19f);
 // are its A operand and come straight from memory, a block ahead).  A lane gets 16 scores of one user per block: its cell
 // is items 8 g + 4 h + 0..3, g = 0..3, of the block.
 //
-// The vector work per score is what bounds this kernel once there are users enough, so the scores are formed in two
-// instructions instead of the definition's four: the accumulator starts at 1.5 * 2^23 as the BITS of a float, so that its
+// The vector work per score is what bounds this kernel once there are users enough, so a score is formed in two
+// instructions instead of the definition's four (its maximum is a third): the accumulator starts at 1.5 * 2^23 as the BITS of a float, so that its
 // bits ARE the float 1.5 * 2^23 + sum (|sum| <= 256 * 2^14 = 2^22), and
 //     v = fma(fma(acc, sp, -1.5 * 2^23 * sp), sq, b).
 // Against the defined score e: the inner step is off by at most half an ulp of 1.5 * 2^23 sp (0.75 sp) and of the result
@@ -110,9 +113,10 @@ static constexpr float NO_SCORE = LOWEST * (1.f - 0x1p-19f);
 // they give: |v - e| <= 1.6 |sp sq| + 2^-22 |v|, plus a few steps of 2^-149.  A cell's bound is its largest v plus that
 // (with 2^-21 for its own rounding), its best e at least the bound less twice that; the first term, which does not show in
 // the bound, is kept per user and slice of the items.
-// 4096 users, 200k items of 64 columns: 125 to 140 us (0.8 * 10^15 operations/s; the vector instructions alone need 75, the
-// matrix instructions 50, and without its stores it takes 100 to 105).  33 users, 2M items of 128 columns: 69 us, 3.9 TB/s, bound
-// by reading the table.
+// 4096 users, 200k items of 64 columns: 125 to 140 us (0.8 * 10^15 operations/s): 3.65 vector instructions a score all in all keep the
+// vector pipes busy 61 % of the cycles, the matrix pipes 17 %, and 285 MB are written, a third more than the bounds are; without
+// its stores it takes 100 to 105.  33 users, 2M items of 128 columns: 69 us, 3.9 TB/s: vector pipes 21 %, the waves wait for the one
+// block each has on its way.
 // Scales above 2^50 (of either sign) could leave float32's range in one form and not in the other: users and blocks that have such scales
 // take the definition itself.
 template <int KS, int UW>
@@ -455,9 +459,12 @@ __device__ __forceinline__ int64_t cell_first(int64_t y) { return (y >> 1) * BLO
 __device__ __forceinline__ int64_t cell_item(int64_t y, int e) { return cell_first(y) + 8 * (e >> 2) + (e & 3); }
 
 // NT = 256 threads, or 1024 where there are few users and one workgroup's time is the call's; LPI: see RowDot.
-// Bound by latency, some twenty dependent steps a user: 4096 users of 200k items 68 to 78 us (five workgroups a CU; more of
-// them at fewer registers gain nothing; with a look at the list's room every 256 items 80), one user of 200k items 12.5 us,
-// 33 of 2M items 20 us (with 256 of the 1024 threads scoring 15 and 25).
+// Some twenty dependent steps a user.  4096 users of 200k items 68 to 78 us (vector pipes busy 60 % of the cycles; five workgroups a
+// CU, more of them at fewer registers gain nothing; with a look at the list's room every 256 items 80), one user of 200k items 12.5 us,
+// 33 of 2M items 20 us (with 256 of the 1024 threads scoring 15 and 25), both bound by latency.
+// A train item takes its slice out of the cut.  Of 1024 slices about 1024 exp(-n / 1024) are left for n train items at random: with
+// some thousands there are fewer than k, or the cut is loose, and the user's workgroup scores many cells or all: one user of 200k
+// items 20 us with 40 train items, 100 with 3000, 187 with 10000.
 template <int NT, int LPI, int LIST>
 __global__ __launch_bounds__(NT) void pick_i8_kernel(MaxArgs m)
 {
