@@ -97,3 +97,19 @@ def test_rows_quantised_onto_what_they_are_made_of_are_refused(dev):
     # only the rows that are read count: the last row of X is not among the first n - 1
     dev.quantize_rows(X[:n - 1], out=QuantRows(buf[4096 + (n - 1) * d * 4:][:(n - 1) * d].view(torch.int8).view(n - 1, d), s[:n - 1], d))
     dev.synchronize()
+
+
+@pytest.mark.parametrize("n,I,k", [(2, 60000, 50), (300, 40000, 20), (2, 60000, 200)])
+def test_lists_of_users_whose_train_items_leave_no_cut(dev, n, I, k):
+    """Thousands of train items: hardly a slice of the items, or none, is without one, so that the cut of the second step is loose or
+    missing and most cells are scored; train items are among the best."""
+    import numpy as np
+    from test_gpu_int8 import check_topk, scores_f32, topk_case
+    Pq, sp, Qq, sq, b, masks = topk_case(I + n + k, n, I, 48, 10)
+    rng = np.random.default_rng(n)
+    best = np.argsort(-scores_f32(Pq[1:2], sp[1:2], Qq, sq, b)[0])
+    masks[0] = np.sort(rng.choice(I, 9000, replace=False))
+    masks[1] = np.sort(np.concatenate([best[:2500], rng.choice(best[2500:], 2500, replace=False)]))
+    if n > 2:
+        masks[2], masks[n - 1] = np.arange(0, I, 3), np.sort(rng.choice(I, 3000, replace=False))
+    check_topk(dev, (Pq, sp, Qq, sq, b, masks), np.arange(n), k)
